@@ -8,6 +8,7 @@
 #include <mutex>
 #include <unordered_map>
 
+#include "bindings.h"
 #include "oslo_kernels.h"
 
 namespace {
@@ -1829,6 +1830,14 @@ Tensor moe_few(const Tensor& x, const Tensor& idx, const Tensor& w, int64_t per_
 }
 
 }  // namespace
+
+namespace oslo_bind {
+int dt_code(const at::Tensor& t) { return ::dt_code(t); }
+void check_rc(int rc, const char* what) { ::check_rc(rc, what); }
+cudaStream_t cur_stream(int kernels) { return ::cur_stream(kernels); }
+int* error_word(int device) { return dev_state(device).err.data_ptr<int>(); }
+int sms(int device) { return dev_state(device).sms; }
+}  // namespace oslo_bind
 
 // Schemas. Kernels that take tensors are registered for the CUDA dispatch key (below), which leaves the Meta /
 // fake-tensor slot free for the shape implementations that oslo_b200/ops/fake_impls.py registers from Python.

@@ -401,6 +401,35 @@ int oslo_gemm_grouped(const void* A, const void* B, void* D, int M, int N, int K
                       const int* group_tiles, int flags, int glu_clamped, float glu_limit, float glu_alpha, int* err_word, int num_sms,
                       cudaStream_t stream);
 
+// ---- sequences in pages and packed sequences (paged_cache.cu, ragged_attention.cu, sampling.cu). Strides in elements; row strides `_sr`,
+// head strides `_sh`, batch strides `_sb`. `table` [B, columns] names a sequence's pages; q8: the pools hold e4m3 values and have scales
+int oslo_paged_append(const void* k, const void* v, long long k_sr, long long k_sh, long long v_sr, long long v_sh, void* k_pages,
+                      void* v_pages, float* k_scale, float* v_scale, const int* table, const int* lengths, const int* offsets,
+                      long long rows, int B, int heads, int D, long long pages, int page, int columns, int dtype, int q8, int* err_word,
+                      int num_sms, cudaStream_t stream);
+int oslo_paged_read(const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, void* k, void* v,
+                    const int* table, const int* offsets, long long rows, int B, int heads, int D, long long pages, int page, int columns,
+                    int dtype, int q8, int* err_word, int num_sms, cudaStream_t stream);
+int oslo_paged_attn(const void* q, long long q_sb, long long q_sh, const void* k_pages, const void* v_pages, const float* k_scale,
+                    const float* v_scale, void* o, const int* table, const int* lengths, int B, int H, int heads, int D, long long pages,
+                    int page, int columns, float scale, int window, int dtype, int q8, int* err_word, int num_sms, cudaStream_t stream);
+// lse [Tq, Hq] may be null; key_offsets are `q_off` again where queries and keys are the same rows
+int oslo_ragged_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* q_off, const int* k_off, int B, int Hq,
+                    int Hk, long long Tq, long long Tk, int D, long long q_sr, long long q_sh, long long k_sr, long long k_sh,
+                    long long v_sr, long long v_sh, long long o_sr, long long o_sh, float scale, int window, int dtype, int* err_word,
+                    cudaStream_t stream);
+// three launches (four where D > 128); delta: workspace [Tq, Hq]
+int oslo_ragged_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, float* delta, void* dq,
+                    void* dk, void* dv, const int* q_off, const int* k_off, int B, int Hq, int Hk, long long Tq, long long Tk, int D,
+                    long long q_sr, long long q_sh, long long k_sr, long long k_sh, long long v_sr, long long v_sh, long long o_sr,
+                    long long o_sh, long long g_sr, long long g_sh, long long dq_sr, long long dq_sh, long long dk_sr, long long dk_sh,
+                    long long dv_sr, long long dv_sh, float scale, int window, int dtype, int* err_word, cudaStream_t stream);
+int oslo_sample_max_vocab(int dtype);
+// temperature, top_k, top_p, min_p: per row, or null and the numbers; uniform fp32 or fp64 in [0, 1); out[row]: the token, -1 for none
+int oslo_sample_tokens(const void* logits, long long ld, const void* uniform, int uniform64, const float* temperature, const int* top_k,
+                       const float* top_p, const float* min_p, double temperature1, int top_k1, double top_p1, double min_p1, long long* out,
+                       int rows, int V, int dtype, int num_sms, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

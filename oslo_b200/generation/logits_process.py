@@ -98,6 +98,19 @@ class TopPLogitsWarper(LogitsWarper):
         return scores.masked_fill(mask, self.filter_value)
 
 
+class MinPLogitsWarper(LogitsWarper):
+    """Tokens whose probability is at least ``min_p`` times the largest."""
+
+    def __init__(self, min_p: float, filter_value: float = -float("inf")) -> None:
+        if not 0 <= min_p <= 1.0:
+            raise ValueError("min_p must be in [0, 1]")
+        self.min_p, self.filter_value = float(min_p), filter_value
+
+    def __call__(self, input_ids, scores):
+        p = torch.exp(scores - scores.amax(dim=-1, keepdim=True))
+        return scores.masked_fill(p < self.min_p, self.filter_value)
+
+
 class NoRepeatNGramLogitsProcessor(LogitsProcessor):
     """Host-side n-gram blocking."""
 

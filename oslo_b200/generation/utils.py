@@ -19,11 +19,12 @@ import torch
 import torch.distributed as dist
 from torch import Tensor
 
+from .. import ops
 from .beam_search import BeamSearchScorer
 from .logits_process import (ForcedBOSTokenLogitsProcessor, ForcedEOSTokenLogitsProcessor,
                              FusedNoRepeatNGramLogitsProcessor, HammingDiversityLogitsProcessor,
                              InfNanRemoveLogitsProcessor, LogitsProcessorList, MaxLengthCriteria, MaxTimeCriteria,
-                             MinLengthLogitsProcessor, NoBadWordsLogitsProcessor, NoRepeatNGramLogitsProcessor,
+                             MinLengthLogitsProcessor, MinPLogitsWarper, NoBadWordsLogitsProcessor, NoRepeatNGramLogitsProcessor,
                              PrefixConstrainedLogitsProcessor, RepetitionPenaltyLogitsProcessor,
                              StoppingCriteriaList, TemperatureLogitsWarper, TopKLogitsWarper, TopPLogitsWarper)
 
@@ -111,7 +112,7 @@ class GenerationMixin:
         return procs
 
     @staticmethod
-    def _get_logits_warper(top_k, top_p, temperature, num_beams) -> LogitsProcessorList:
+    def _get_logits_warper(top_k, top_p, temperature, num_beams, min_p=None) -> LogitsProcessorList:
         warpers = LogitsProcessorList()
         keep = 2 if num_beams > 1 else 1
         if temperature is not None and temperature != 1.0:
@@ -120,6 +121,8 @@ class GenerationMixin:
             warpers.append(TopKLogitsWarper(top_k, min_tokens_to_keep=keep))
         if top_p is not None and top_p < 1.0:
             warpers.append(TopPLogitsWarper(top_p, min_tokens_to_keep=keep))
+        if min_p:
+            warpers.append(MinPLogitsWarper(min_p))
         return warpers
 
     # ------------------------------------------------------------------ entry point
@@ -143,10 +146,16 @@ class GenerationMixin:
                  forced_bos_token_id: Optional[int] = None, forced_eos_token_id: Optional[int] = None,
                  remove_invalid_values: Optional[bool] = None, synced_gpus: bool = False,
                  fused_no_repeat_ngram_blocking: Optional[bool] = None, use_static_cache: bool = True,
-                 cuda_graph: bool = False, **model_kwargs) -> Union[Tensor, GenerateOutput]:
+                 cuda_graph: bool = False, min_p: Optional[float] = None, fused_sampling: bool = False,
+                 **model_kwargs) -> Union[Tensor, GenerateOutput]:
         """``cuda_graph=True`` (not in the reference) runs plain greedy decoding - one beam, no sampling, no logits
         processors, no attention mask - through ``GraphedGreedyDecoder``: eager prefill, then one CUDA-graph replay per
         token. Any other combination ignores the flag.
+
+        ``fused_sampling=True`` (not in the reference): with ``do_sample`` and one beam, temperature, top-k, top-p, min-p and the draw run in
+        ``ops.sample_tokens``, one kernel a token, with ``torch.rand`` numbers. The distribution is the warpers', but for logits that are
+        equal at a border (ranked by index here); the tokens of a seed are others than without it. ``min_p`` keeps tokens of at least
+        that share of the largest probability, one beam only.
 
         ``output_attentions`` / ``output_hidden_states`` with ``return_dict_in_generate=True`` add ``attentions`` /
         ``hidden_states`` to the result: one entry per generated token, each a tuple over the layers, as the reference's
@@ -235,9 +244,10 @@ class GenerationMixin:
                 return self._graph_greedy(input_ids, max_length, pad_token_id, eos_token_id, return_dict_in_generate)
             return self.greedy_search(input_ids, procs, stops, **common, **model_kwargs)
         if num_beams == 1 and do_sample:
-            warper = self._get_logits_warper(top_k, top_p, temperature, num_beams)
+            warper = self._get_logits_warper(top_k, top_p, temperature, num_beams, min_p)
             input_ids, model_kwargs = self._expand_inputs_for_generation(input_ids, num_return_sequences, **model_kwargs)
-            return self.sample(input_ids, procs, stops, warper, **common, **model_kwargs)
+            fused = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p or 0.0) if fused_sampling else None
+            return self.sample(input_ids, procs, stops, warper, fused_settings=fused, **common, **model_kwargs)
         bsz = input_ids.shape[0]
         if num_return_sequences > num_beams:
             raise ValueError("num_return_sequences must be <= num_beams")
@@ -330,7 +340,7 @@ class GenerationMixin:
 
     def sample(self, input_ids, logits_processor=None, stopping_criteria=None, logits_warper=None,
                pad_token_id=None, eos_token_id=None, output_scores=False, return_dict_in_generate=False,
-               synced_gpus=False, **model_kwargs):
+               synced_gpus=False, fused_settings=None, **model_kwargs):
         procs = logits_processor or LogitsProcessorList()
         stops = stopping_criteria or StoppingCriteriaList()
         warper = logits_warper or LogitsProcessorList()
@@ -338,10 +348,17 @@ class GenerationMixin:
         unfinished = input_ids.new_ones(input_ids.shape[0])
         while True:
             out, logits = self._step_logits(input_ids, model_kwargs)
-            s = warper(input_ids, procs(input_ids, logits))
+            s = procs(input_ids, logits)
+            if fused_settings is not None:
+                nxt = ops.sample_tokens(s, torch.rand(s.size(0), device=s.device), **fused_settings)
+                if bool((nxt < 0).any()):
+                    raise RuntimeError("the logits hold no token to sample: not a number, or all minus infinity")
+            if fused_settings is None or scores is not None:
+                s = warper(input_ids, s)
             if scores is not None:
                 scores.append(s)
-            nxt = torch.multinomial(torch.softmax(s, dim=-1), num_samples=1).squeeze(1)
+            if fused_settings is None:
+                nxt = torch.multinomial(torch.softmax(s, dim=-1), num_samples=1).squeeze(1)
             if eos_token_id is not None:
                 nxt = nxt * unfinished + pad_token_id * (1 - unfinished)
                 unfinished = unfinished.mul((nxt != eos_token_id).long())

@@ -73,7 +73,7 @@ from .functional import (  # noqa: E402
     ban_repeated_ngrams, decode_attention, rms_norm, residual_join, silu_mul, gated_recurrence, sink_attention,
     latent_decode, moe_route, moe_experts, linear_fp32, stacked_linear, branch_join, clamped_glu, gated_rms_norm,
     decayed_attention, bonus_recurrence, token_shift, causal_conv, selective_scan, matrix_memory, hyper_join,
-    token_gate,
+    token_gate, ragged_attention, paged_append, paged_read, paged_attention, sample_tokens,
 )
 
 __all__ = [
@@ -83,5 +83,5 @@ __all__ = [
     "decode_attention", "rms_norm", "residual_join", "silu_mul", "gated_recurrence", "sink_attention", "latent_decode",
     "moe_route", "moe_experts", "linear_fp32", "stacked_linear", "branch_join", "clamped_glu", "gated_rms_norm",
     "decayed_attention", "bonus_recurrence", "token_shift", "causal_conv", "selective_scan", "matrix_memory",
-    "hyper_join", "token_gate",
+    "hyper_join", "token_gate", "ragged_attention", "paged_append", "paged_read", "paged_attention", "sample_tokens",
 ]

@@ -1135,3 +1135,70 @@ def moe_experts(h: Tensor, idx: Tensor, up: Tensor, down: Tensor, unit: str = "r
     slots, rows, tile_group, n_tiles = _ext().moe_plan(_rows(h), idx, up.size(0), scale)
     a = _ext().moe_grouped(rows, up, tile_group, n_tiles, u, float(limit), float(alpha))
     return _ext().moe_grouped(a, down, tile_group, n_tiles, 0), slots
+
+
+# ---------------------------------------------------------------------------------------------------------------
+def _packed_heads(t: Tensor) -> Tensor:
+    """``[rows, heads, D]`` as the kernels of packed and paged sequences read it: contiguous D, 16-byte aligned heads inside their row."""
+    r, h, d = t.stride()
+    if d != 1 or r % 8 or h % 8 or t.data_ptr() % 16 or (h > r and t.size(0) > 1 and t.size(1) > 1) or (h <= 0 and t.size(1) > 1) or (r <= 0 and t.size(0) > 1):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def ragged_ok(q: Tensor, k: Tensor, v: Tensor) -> bool:
+    return q.dtype in _16BIT and k.dtype == q.dtype and v.dtype == q.dtype and q.dim() == 3 and q.size(2) % 8 == 0 and q.size(2) <= 256
+
+
+class _Ragged(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offsets, key_offsets, scale, window):
+        q, k, v = _packed_heads(q), _packed_heads(k), _packed_heads(v)
+        o, lse = _ext().ragged_fwd(q, k, v, offsets, key_offsets, scale, window, True)
+        ctx.save_for_backward(q, k, v, o, lse, offsets, key_offsets)
+        ctx.cfg = (scale, window)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, offsets, key_offsets = ctx.saved_tensors
+        dq, dk, dv = _ext().ragged_bwd(_packed_heads(do), q, k, v, o, lse, offsets, key_offsets, *ctx.cfg)
+        return dq, dk, dv, None, None, None, None
+
+
+def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offsets: Tensor, window: Optional[int], scale: float) -> Tensor:
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Ragged.apply(q, k, v, offsets, key_offsets, float(scale), int(window or 0))
+    return _ext().ragged_fwd(_packed_heads(q), _packed_heads(k), _packed_heads(v), offsets, key_offsets, scale, window or 0, False)[0]
+
+
+def paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale) -> None:
+    _ext().paged_append(_packed_heads(k.detach()), _packed_heads(v.detach()), k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)
+
+
+def paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype):
+    if dtype is None:
+        dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
+    return _ext().paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype)
+
+
+def paged_attention(q, k_pages, v_pages, page_table, lengths, window, scale, k_scale, v_scale) -> Tensor:
+    return _ext().paged_attn(_packed_heads(q.detach()), k_pages, v_pages, page_table, lengths, scale, window or 0, k_scale, v_scale)
+
+
+def sample_ok(logits: Tensor) -> bool:
+    """Whether a row fits the shared memory of a cluster of eight blocks."""
+    return logits.dim() == 2 and logits.dtype in (torch.float32,) + _16BIT and logits.size(1) * logits.element_size() <= 1600000
+
+
+def sample_tokens(logits, uniform, temperature, top_k, top_p, min_p) -> Tensor:
+    x = logits.detach()
+    if x.stride(1) != 1 and x.size(1) > 1:
+        x = x.contiguous()
+    tensors, numbers = [], []
+    for value, default in ((temperature, 1.0), (top_k, 0), (top_p, 1.0), (min_p, 0.0)):
+        own = isinstance(value, Tensor)
+        tensors.append(value if own else None)
+        numbers.append(default if own else value)
+    return _ext().sample_tokens(x, uniform, *tensors, *numbers)

@@ -345,3 +345,28 @@ def register() -> None:
     @reg("oslo_b200::scan_step")
     def _(x, dt, w_dt, dt_bias, a_log, b, c, d, z, keep, state):
         return x.new_empty(x.shape)
+
+    @reg("oslo_b200::ragged_fwd")
+    def _(q, k, v, offsets, key_offsets, scale, window, with_lse):
+        return q.new_empty(q.shape), q.new_empty(q.shape[:2] if with_lse else (0,), dtype=torch.float32)
+
+    @reg("oslo_b200::ragged_bwd")
+    def _(dout, q, k, v, o, lse, offsets, key_offsets, scale, window):
+        return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+    @reg("oslo_b200::paged_append")
+    def _(k, v, k_pages, v_pages, table, lengths, offsets=None, k_scale=None, v_scale=None):
+        return None
+
+    @reg("oslo_b200::paged_read")
+    def _(k_pages, v_pages, table, offsets, tokens, k_scale, v_scale, dtype):
+        shape = (tokens, k_pages.size(1), k_pages.size(3))
+        return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+    @reg("oslo_b200::paged_attn")
+    def _(q, k_pages, v_pages, table, lengths, scale, window, k_scale=None, v_scale=None):
+        return q.new_empty(q.shape)
+
+    @reg("oslo_b200::sample_tokens")
+    def _(logits, uniform, temperature, top_k, top_p, min_p, temperature1, top_k1, top_p1, min_p1):
+        return logits.new_empty((logits.size(0),), dtype=torch.int64)

@@ -363,3 +363,84 @@ def selective_scan(x: Tensor, dt: Tensor, dt_bias: Tensor, a_log: Tensor, b: Ten
     if state is not None:
         state.copy_(final.detach())
     return y
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Sequences of different lengths: packed behind one another, or in the pages of a shared pool.
+def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offsets: Optional[Tensor] = None, window: Optional[int] = None,
+                     scale: Optional[float] = None) -> Tensor:
+    """Causal attention of packed sequences with grouped heads: ``q`` ``[T, heads, D]``, ``k`` and ``v`` ``[T_k, kv_heads, D]``.
+
+    Sequence ``b`` has the rows ``offsets[b]`` to ``offsets[b + 1] - 1`` (int32 ``[B + 1]`` on the device, not decreasing; the host never
+    reads them) of ``q``, and those of ``key_offsets`` (default: the same) of ``k`` and ``v``; its last query stands at its last key, so
+    cached keys may lie ahead of a prompt that goes on. ``window``: a query sees that many keys, its own place among them. Rows of no
+    sequence, and queries that see no key, give zeros. 16-bit CUDA tensors with ``D`` a multiple of 8 up to 256 take the tcgen05
+    kernels, forward and backward; sequences do not touch each other's numbers, whatever those are (a number that is none spoils rows of its own
+    sequence only)."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.size(-1))
+    if _k(q):
+        from . import cuda_ops
+        if cuda_ops.ragged_ok(q, k, v):
+            return cuda_ops.ragged_attention(q, k, v, offsets, offsets if key_offsets is None else key_offsets, window, scale)
+    return ref.ragged_attention(q, k, v, offsets, key_offsets, window, scale)
+
+
+def paged_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths: Tensor, offsets: Optional[Tensor] = None,
+                 k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None) -> None:
+    """New keys and values ``[T, kv_heads, D]`` into a paged cache, in place.
+
+    The pools ``k_pages`` and ``v_pages`` are ``[pages, kv_heads, page, D]`` in the keys' type, or ``float8_e4m3fn`` with the fp32 scales
+    ``k_scale`` and ``v_scale`` ``[pages, kv_heads, page]`` (a vector's largest magnitude over 448). ``page_table`` (int32
+    ``[B, columns]``) names a sequence's pages in order; ``lengths`` (int32 ``[B]``) counts its tokens, the new ones among them.
+    Sequence ``b``'s new tokens are the rows ``offsets[b]`` to ``offsets[b + 1] - 1``, its last ones (``None``: one row per sequence).
+    A sequence without a length, a position without a page and rows of no sequence are passed over. No gradients."""
+    if _k(k):
+        from . import cuda_ops
+        return cuda_ops.paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)
+    return ref.paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)
+
+
+def paged_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, offsets: Tensor, tokens: int, k_scale: Optional[Tensor] = None,
+               v_scale: Optional[Tensor] = None, dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
+    """The keys and values ``[tokens, kv_heads, D]`` that a paged cache holds (see ``paged_append``), sequence behind sequence: the rows
+    ``offsets[b]`` to ``offsets[b + 1] - 1`` are the first tokens of sequence ``b``, as ``ragged_attention`` takes them. ``dtype``: the
+    result's type where the pools are 8-bit. Rows without a page give zeros."""
+    if _k(k_pages):
+        from . import cuda_ops
+        return cuda_ops.paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype)
+    return ref.paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype)
+
+
+def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths: Tensor, window: Optional[int] = None,
+                    scale: Optional[float] = None, k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None) -> Tensor:
+    """Attention of one new token per sequence, ``q`` ``[B, heads, D]``, over a paged cache (see ``paged_append``): the first
+    ``lengths[b]`` tokens of sequence ``b``, or the last ``window`` of them. Sequences may share pages. A sequence of no tokens gives
+    zeros; tokens without a page are passed over. No gradients."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.size(-1))
+    if _k(q):
+        from . import cuda_ops
+        return cuda_ops.paged_attention(q, k_pages, v_pages, page_table, lengths, window, scale, k_scale, v_scale)
+    return ref.paged_attention(q, k_pages, v_pages, page_table, lengths, window, scale, k_scale, v_scale)
+
+
+def sample_tokens(logits: Tensor, uniform: Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Tensor:
+    """A token per row of ``logits`` ``[rows, vocab]``, chosen by ``uniform`` ``[rows]`` (fp32 or fp64, in ``[0, 1)``); int64 ``[rows]``.
+
+    Tokens are ranked by logit, equal ones by index. With ``w = exp((logit - largest) / temperature)``: ``top_k`` (0: all) keeps that
+    many ranks, ``top_p`` those of them whose lower ranks have at most this share of their mass, ``min_p`` tokens of at least this
+    ``w``; rank 0 always stays. The first token, by index, whose kept mass together with its predecessors' exceeds ``uniform`` times
+    the whole is the choice. Every setting is a number or a tensor ``[rows]`` (fp32; ``top_k`` int32). A temperature of 0 takes the
+    largest logit. A row whose logits hold no number to choose (one that is no number, or only minus infinities), or whose ``uniform``
+    is outside ``[0, 1)``, gives -1. No gradients."""
+    for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+        if not isinstance(value, Tensor) and not value >= 0:
+            raise ValueError(f"sample_tokens: {name} must not be negative")
+    if not logits.is_floating_point():
+        raise ValueError("sample_tokens: logits must be floating-point numbers")
+    if _k(logits):
+        from . import cuda_ops
+        if cuda_ops.sample_ok(logits):
+            return cuda_ops.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
+    return ref.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)

@@ -693,3 +693,183 @@ def selective_scan(x: Tensor, dt: Tensor, dt_bias: Tensor, a_log: Tensor, b: Ten
         out.append(torch.einsum("bcn,bn->bc", s, cf[:, t]))
     y = torch.stack(out, dim=1) + d.to(torch.float32) * xf
     return (y.reshape(x.shape) * F.silu(z.to(torch.float32))).to(x.dtype), s
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Packed and paged sequences
+FP8_MAX = 448.0              # largest e4m3 value
+
+
+def _sequence_of(offsets: Tensor, rows: int) -> Tuple[Tensor, Tensor]:
+    """Sequence of every packed row and its place there; sequence -1 for rows of none."""
+    at = torch.arange(rows, device=offsets.device)
+    off = offsets.to(torch.long)
+    seq = torch.searchsorted(off, at, right=True) - 1
+    seq = torch.where((at >= off[0]) & (at < off[-1]), seq, -1)
+    return seq, at - off[seq.clamp(min=0)]
+
+
+def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offsets: Optional[Tensor], window: Optional[int],
+                     scale: float) -> Tensor:
+    """See ``functional.ragged_attention``; scores of all rows with all keys."""
+    if q.dim() != 3 or k.shape != v.shape or k.dim() != 3 or k.size(2) != q.size(2) or k.size(1) == 0 or q.size(1) % k.size(1):
+        raise ValueError("ragged_attention: q must be [T, heads, D], k and v [T_k, kv_heads, D] with kv_heads a divisor of heads")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("ragged_attention: q, k and v must have one type")
+    key_offsets = offsets if key_offsets is None else key_offsets
+    if offsets.dtype != torch.int32 or key_offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 2 or key_offsets.shape != offsets.shape:
+        raise ValueError("ragged_attention: offsets are int32 [sequences + 1]")
+    if not scale > 0 or (window is not None and window < 0):
+        raise ValueError("ragged_attention: the scale must be positive and the window not negative")
+    qs, qi = _sequence_of(offsets, q.size(0))
+    ks, ki = _sequence_of(key_offsets, k.size(0))
+    lens, klens = (o[1:].to(torch.long) - o[:-1].to(torch.long) for o in (offsets, key_offsets))
+    at = qi + (klens - lens)[qs.clamp(min=0)]
+    seen = (qs[:, None] == ks[None]) & (qs >= 0)[:, None] & (ki[None] <= at[:, None])
+    if window:
+        seen &= ki[None] > (at - window)[:, None]
+    group = q.size(1) // k.size(1)
+    kf, vf = (t.float().repeat_interleave(group, dim=1).transpose(0, 1) for t in (k, v))
+    s = torch.matmul(q.float().transpose(0, 1), kf.transpose(1, 2)) * scale
+    p = torch.softmax(s.masked_fill(~seen, float("-inf")), dim=-1)
+    p = torch.where(seen & seen.any(-1, keepdim=True), p, torch.zeros((), dtype=p.dtype, device=p.device))
+    return torch.matmul(p, vf).transpose(0, 1).to(q.dtype)
+
+
+def quantise(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """Vectors as e4m3 values and the fp32 number that multiplies them: largest magnitude over 448."""
+    x = x.float()
+    scale = x.abs().amax(-1) * torch.tensor(1.0 / FP8_MAX, dtype=torch.float32)     # one rounding on every device
+    scale = torch.where(torch.isfinite(scale), scale, float("nan"))
+    return (x / torch.where(scale == 0, 1.0, scale)[..., None]).to(torch.float8_e4m3fn), scale
+
+
+def _check_pages(op: str, k_pages, v_pages, page_table, k_scale, v_scale) -> None:
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError(f"{op}: the pools must be two contiguous [pages, heads, page, D] tensors of one type")
+    small = k_pages.dtype == torch.float8_e4m3fn
+    for s in (k_scale, v_scale):
+        if (s is not None) != small or (small and (s.shape != k_pages.shape[:3] or s.dtype != torch.float32 or not s.is_contiguous())):
+            raise ValueError(f"{op}: e4m3 pools have fp32 scales [pages, heads, page], others have none")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.numel() == 0:
+        raise ValueError(f"{op}: the page table must be int32 [sequences, pages of one]")
+
+
+def _place(k_pages: Tensor, page_table: Tensor, seq: Tensor, at: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+    """Page, row in it and whether there is one, of position ``at`` of sequence ``seq``."""
+    page = k_pages.size(2)
+    ok = (seq >= 0) & (at >= 0) & (at < page_table.size(1) * page)
+    at = torch.where(ok, at, 0)
+    pages = page_table.to(torch.long)[seq.clamp(min=0), at // page]
+    ok = ok & (pages >= 0) & (pages < k_pages.size(0))
+    return torch.where(ok, pages, 0), at % page, ok
+
+
+def _stored(pool: Tensor, scale: Optional[Tensor], pages: Tensor, place: Tensor) -> Tensor:
+    """Vectors ``[n, heads, D]`` in 32 bits."""
+    if scale is None:
+        return pool[pages, :, place].float()
+    return pool.view(torch.uint8)[pages, :, place].view(torch.float8_e4m3fn).float() * scale[pages, :, place][..., None]
+
+
+@torch.no_grad()
+def paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale) -> None:
+    """See ``functional.paged_append``."""
+    _check_pages("paged_append", k_pages, v_pages, page_table, k_scale, v_scale)
+    b = page_table.size(0)
+    if k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (k_pages.size(1), k_pages.size(3)) or k.dtype != v.dtype:
+        raise ValueError("paged_append: k and v must be [rows, heads, D] like the pools")
+    if k_scale is None and k.dtype != k_pages.dtype:
+        raise ValueError("paged_append: a pool holds e4m3 values or the type of its keys and values")
+    if lengths.dtype != torch.int32 or lengths.shape != (b,) or (offsets is not None and (offsets.dtype != torch.int32 or offsets.shape != (b + 1,))):
+        raise ValueError("paged_append: lengths are int32 [sequences], offsets int32 [sequences + 1]")
+    if offsets is None and k.size(0) != b:
+        raise ValueError("paged_append: one row per sequence, or offsets")
+    offsets = torch.arange(b + 1, device=k.device) if offsets is None else offsets.to(torch.long)
+    seq, i = _sequence_of(offsets, k.size(0))
+    s0 = seq.clamp(min=0)
+    pages, place, ok = _place(k_pages, page_table, seq, lengths.to(torch.long)[s0] - (offsets[1:] - offsets[:-1])[s0] + i)
+    pages, place = pages[ok], place[ok]
+    for x, pool, scale in ((k, k_pages, k_scale), (v, v_pages, v_scale)):
+        x = x[ok]
+        if scale is None:
+            pool[pages, :, place] = x
+        else:
+            x, s = quantise(x)
+            scale[pages, :, place] = s
+            pool.view(torch.uint8)[pages, :, place] = x.view(torch.uint8)
+
+
+@torch.no_grad()
+def paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype) -> Tuple[Tensor, Tensor]:
+    """See ``functional.paged_read``."""
+    _check_pages("paged_read", k_pages, v_pages, page_table, k_scale, v_scale)
+    if offsets.dtype != torch.int32 or offsets.shape != (page_table.size(0) + 1,) or tokens < 0:
+        raise ValueError("paged_read: offsets are int32 [sequences + 1]")
+    if k_scale is None and dtype is not None and dtype != k_pages.dtype:
+        raise ValueError("paged_read: a pool holds e4m3 values or the type of its keys and values")
+    dtype = (torch.bfloat16 if k_scale is not None else k_pages.dtype) if dtype is None else dtype
+    seq, at = _sequence_of(offsets, tokens)
+    pages, place, ok = _place(k_pages, page_table, seq, at)
+    return tuple(torch.where(ok[:, None, None], _stored(pool, scale, pages, place), 0.0).to(dtype)
+                 for pool, scale in ((k_pages, k_scale), (v_pages, v_scale)))
+
+
+@torch.no_grad()
+def paged_attention(q, k_pages, v_pages, page_table, lengths, window, scale, k_scale, v_scale) -> Tensor:
+    """See ``functional.paged_attention``."""
+    _check_pages("paged_attention", k_pages, v_pages, page_table, k_scale, v_scale)
+    b, kv = page_table.size(0), k_pages.size(1)
+    if q.dim() != 3 or q.size(0) != b or q.size(2) != k_pages.size(3) or q.size(1) % kv:
+        raise ValueError("paged_attention: q must be [sequences, heads, D]")
+    if k_scale is None and q.dtype != k_pages.dtype:
+        raise ValueError("paged_attention: a pool holds e4m3 values or the type of the queries")
+    if lengths.dtype != torch.int32 or lengths.shape != (b,) or (window is not None and window < 0):
+        raise ValueError("paged_attention: lengths are int32 [sequences], and the window is not negative")
+    room = page_table.size(1) * k_pages.size(2)
+    lens = lengths.to(torch.long).clamp(0, room)
+    at = torch.arange(room, device=q.device)
+    seq = torch.arange(b, device=q.device)[:, None].expand(b, room)
+    pages, place, ok = _place(k_pages, page_table, seq, at.expand(b, room))
+    ok = ok & (at < lens[:, None])
+    if window:
+        ok = ok & (at >= (lens - window)[:, None])
+    k, v = (_stored(pool, s, pages.reshape(-1), place.reshape(-1)).view(b, room, kv, -1).transpose(1, 2) for pool, s in ((k_pages, k_scale), (v_pages, v_scale)))
+    v = torch.where(ok[:, None, :, None], v, 0.0)
+    s = torch.matmul(q.float().unflatten(1, (kv, -1)), k.transpose(2, 3)) * scale
+    p = torch.softmax(s.masked_fill(~ok[:, None, None], float("-inf")), dim=-1)
+    p = torch.where(ok.any(1)[:, None, None, None] & ok[:, None, None], p, 0.0)
+    return torch.matmul(p, v).flatten(1, 2).to(q.dtype)
+
+
+@torch.no_grad()
+def sample_tokens(logits, uniform, temperature, top_k, top_p, min_p) -> Tensor:
+    """See ``functional.sample_tokens``; sums in 64 bits."""
+    if logits.dim() != 2 or logits.size(1) == 0:
+        raise ValueError("sample_tokens: logits must be [rows, vocabulary]")
+    rows, vocab = logits.shape
+    if uniform.dtype not in (torch.float32, torch.float64) or uniform.shape != (rows,):
+        raise ValueError("sample_tokens: uniform must be fp32 or fp64 [rows]")
+
+    def per_row(value, dtype, name):
+        if isinstance(value, Tensor) and (value.shape != (rows,) or value.dtype != dtype):
+            raise ValueError(f"sample_tokens: {name} must be a number or {dtype} [rows]")
+        return torch.as_tensor(value, dtype=torch.float64, device=logits.device).reshape(-1, 1)
+
+    t, p, low = (per_row(x, torch.float32, n) for x, n in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")))
+    k = per_row(top_k, torch.int32, "top_k")
+    x = logits.double()
+    top = x.amax(1, keepdim=True)
+    rank = torch.arange(vocab, device=x.device)[None]
+    order = torch.sort(x, dim=1, descending=True, stable=True).indices
+    w = torch.where(x == top, 1.0, torch.exp(torch.where(x == top, 0.0, x - top) / torch.where(t > 0, t, 1.0)))
+    ranked = torch.gather(w, 1, order) * ((k <= 0) | (rank < k))
+    before = torch.cumsum(ranked, 1) - ranked
+    keep = (ranked >= low.clamp(max=1.0)) & ((p >= 1) | (before <= p * ranked.sum(1, keepdim=True)))
+    keep = torch.where(t > 0, keep | (rank == 0), rank == 0)
+    mass = torch.zeros_like(w).scatter_(1, order, torch.where(keep, ranked, 0.0))
+    sums = torch.cumsum(mass, 1)
+    u = uniform.double()[:, None]
+    token = (sums <= u * sums[:, -1:]).sum(1).clamp(max=vocab - 1)
+    good = ~torch.isnan(x).any(1) & (top[:, 0] > float("-inf")) & (u[:, 0] >= 0) & (u[:, 0] < 1)
+    return torch.where(good, token, -1)
