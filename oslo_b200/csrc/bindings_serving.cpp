@@ -17,36 +17,36 @@ void check_ints(const Tensor& t, const Tensor& like, int64_t numel, const char* 
   TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == numel, op, ": ", name,
               " must be ", numel, " contiguous int32 numbers on ", like.device());
 }
-// [rows, heads, D] with contiguous, 16-byte aligned heads
-void check_rows(const Tensor& t, const char* op, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 3 && (t.size(2) == 1 || t.stride(2) == 1) && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-                  t.size(2) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              op, ": ", name, " must be [rows, heads, D] with contiguous D (a multiple of 8) and 16-byte aligned heads");
+// [rows, heads, D] as the kernels read it: contiguous D, 16-byte aligned heads inside their row; a copy of what is laid out otherwise
+Tensor rows_of(const Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 3 && t.size(2) % 8 == 0, op, ": ", name, " must be [rows, heads, D] with D a multiple of 8");
   TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, op, ": ", name, " must be bf16 or fp16");
+  const int64_t r = t.stride(0), h = t.stride(1);
+  const bool one_row = t.size(0) <= 1, one_head = t.size(1) <= 1;
+  const bool good = t.stride(2) == 1 && (one_row || r % 8 == 0) && (one_head || h % 8 == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                    (one_row || r > 0) && (one_head || h > 0) && (one_row || one_head || r >= h);
+  return good ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 // ------------------------------------------------------------------------------------------------------------------ packed sequences
 void check_ragged(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& off, const Tensor& koff, int64_t window, double scale) {
-  check_rows(q, "ragged_attention", "q");
-  check_rows(k, "ragged_attention", "k");
-  check_rows(v, "ragged_attention", "v");
-  TORCH_CHECK(k.sizes() == v.sizes() && k.size(2) == q.size(2) && k.size(1) > 0 && q.size(1) % k.size(1) == 0 && q.size(2) <= 256 &&
-                  k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() && v.device() == q.device(),
-              "ragged_attention: q, k and v do not match");
-  for (const Tensor* t : {&q, &k, &v})      // tensor maps: the head's stride inside the row's
-    TORCH_CHECK(t->size(1) == 1 || t->size(0) == 1 || (t->stride(1) > 0 && t->stride(0) >= t->stride(1)), "ragged_attention: heads must lie inside the rows");
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(2) == q.size(2) && k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0 && q.size(2) > 0 &&
+                  q.size(2) <= 256 && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() &&
+                  v.device() == q.device(), "ragged_attention: q, k and v do not match");
   TORCH_CHECK(off.numel() >= 2, "ragged_attention: offsets must hold a sequence's start and end at least");
   check_ints(off, q, off.numel(), "ragged_attention", "offsets");
   check_ints(koff, q, off.numel(), "ragged_attention", "key_offsets");
   TORCH_CHECK(window >= 0 && window <= 0x7fffffff && scale > 0.0, "ragged_attention: the window must not be negative and the scale must be positive");
 }
 
-std::tuple<Tensor, Tensor> ragged_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& off, const Tensor& koff, double scale,
+std::tuple<Tensor, Tensor> ragged_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& off, const Tensor& koff, double scale,
                                       int64_t window, bool with_lse) {
+  TORCH_CHECK(q_.is_cuda(), "ragged_attention: q must be on a GPU");
+  c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = rows_of(q_, "ragged_attention", "q"), k = rows_of(k_, "ragged_attention", "k"), v = rows_of(v_, "ragged_attention", "v");
   check_ragged(q, k, v, off, koff, window, scale);
-  c10::cuda::CUDAGuard guard(q.device());
   Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-  Tensor lse = with_lse ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
+  Tensor lse = at::empty({with_lse ? q.size(0) : 0, q.size(1)}, q.options().dtype(at::kFloat));
   if (q.numel() == 0) return {o, lse};
   if (k.size(0) == 0) {                      // nothing to see
     o.zero_();
@@ -61,15 +61,16 @@ std::tuple<Tensor, Tensor> ragged_fwd(const Tensor& q, const Tensor& k, const Te
   return {o, lse};
 }
 
-std::tuple<Tensor, Tensor, Tensor> ragged_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
+std::tuple<Tensor, Tensor, Tensor> ragged_bwd(const Tensor& dout_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o,
                                               const Tensor& lse, const Tensor& off, const Tensor& koff, double scale, int64_t window) {
+  TORCH_CHECK(q_.is_cuda(), "ragged_attention: q must be on a GPU");
+  c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = rows_of(q_, "ragged_attention", "q"), k = rows_of(k_, "ragged_attention", "k"), v = rows_of(v_, "ragged_attention", "v");
+  const Tensor dout = rows_of(dout_, "ragged_attention", "the output's gradient");
   check_ragged(q, k, v, off, koff, window, scale);
-  check_rows(o, "ragged_attention", "the output");
-  check_rows(dout, "ragged_attention", "the output's gradient");
-  TORCH_CHECK(o.sizes() == q.sizes() && dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() && o.scalar_type() == q.scalar_type() &&
-                  dout.device() == q.device() && lse.numel() == q.size(0) * q.size(1), "ragged_attention: the output and its gradient must be like q");
-  TORCH_CHECK(dout.size(1) == 1 || dout.size(0) == 1 || (dout.stride(1) > 0 && dout.stride(0) >= dout.stride(1)), "ragged_attention: heads must lie inside the rows");
-  c10::cuda::CUDAGuard guard(q.device());
+  TORCH_CHECK(o.sizes() == q.sizes() && o.is_contiguous() && dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() &&
+                  o.scalar_type() == q.scalar_type() && dout.device() == q.device() && lse.numel() == q.size(0) * q.size(1),
+              "ragged_attention: the output and its gradient must be like q");
   // gradients of slices of one projection's rows are slices of one tensor too, so that nobody has to join them
   const int64_t D = q.size(2), Wq = q.size(1) * D, Wk = k.size(1) * D, W = Wq + 2 * Wk;
   Tensor dq, dk, dv;
@@ -131,10 +132,11 @@ Pool check_pool(const char* op, const Tensor& kp, const Tensor& vp, const option
 }
 float* scale_ptr(const optional<Tensor>& t) { return given(t) ? t->data_ptr<float>() : nullptr; }
 
-void paged_append(const Tensor& k, const Tensor& v, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lengths,
+void paged_append(const Tensor& k_, const Tensor& v_, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lengths,
                   const optional<Tensor>& offsets, const optional<Tensor>& ks, const optional<Tensor>& vs) {
-  check_rows(k, "paged_append", "k");
-  check_rows(v, "paged_append", "v");
+  TORCH_CHECK(k_.is_cuda(), "paged_append: k must be on a GPU");
+  c10::cuda::CUDAGuard guard(k_.device());
+  const Tensor k = rows_of(k_, "paged_append", "k"), v = rows_of(v_, "paged_append", "v");
   const Pool p = check_pool("paged_append", kp, vp, ks, vs, table, k, k.scalar_type());
   TORCH_CHECK(k.sizes() == v.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device() && k.size(1) == p.heads && k.size(2) == p.D,
               "paged_append: k and v must be [rows, heads, D] like the pools");
@@ -142,7 +144,6 @@ void paged_append(const Tensor& k, const Tensor& v, const Tensor& kp, const Tens
   if (given(offsets)) check_ints(*offsets, k, p.B + 1, "paged_append", "offsets");
   else TORCH_CHECK(k.size(0) == p.B, "paged_append: one row per sequence, or offsets");
   if (k.size(0) == 0) return;
-  c10::cuda::CUDAGuard guard(k.device());
   check_rc(oslo_paged_append(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), kp.data_ptr(), vp.data_ptr(), scale_ptr(ks),
                              scale_ptr(vs), table.data_ptr<int>(), lengths.data_ptr<int>(), given(offsets) ? offsets->data_ptr<int>() : nullptr, k.size(0),
                              static_cast<int>(p.B), static_cast<int>(p.heads), static_cast<int>(p.D), p.pages, static_cast<int>(p.page),
@@ -164,14 +165,15 @@ std::tuple<Tensor, Tensor> paged_read(const Tensor& kp, const Tensor& vp, const 
   return {k, v};
 }
 
-Tensor paged_attn(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lengths, double scale, int64_t window,
+Tensor paged_attn(const Tensor& q_, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lengths, double scale, int64_t window,
                   const optional<Tensor>& ks, const optional<Tensor>& vs) {
-  check_rows(q, "paged_attention", "q");
+  TORCH_CHECK(q_.is_cuda(), "paged_attention: q must be on a GPU");
+  c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = rows_of(q_, "paged_attention", "q");
   const Pool p = check_pool("paged_attention", kp, vp, ks, vs, table, q, q.scalar_type());
   TORCH_CHECK(q.size(0) == p.B && q.size(1) > 0 && q.size(1) % p.heads == 0 && q.size(2) == p.D, "paged_attention: q must be [sequences, heads, D]");
   TORCH_CHECK(window >= 0 && window <= 0x7fffffff, "paged_attention: the window must not be negative");
   check_ints(lengths, q, p.B, "paged_attention", "lengths");
-  c10::cuda::CUDAGuard guard(q.device());
   Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   check_rc(oslo_paged_attn(q.data_ptr(), q.stride(0), q.stride(1), kp.data_ptr(), vp.data_ptr(), scale_ptr(ks), scale_ptr(vs), o.data_ptr(),
                            table.data_ptr<int>(), lengths.data_ptr<int>(), static_cast<int>(p.B), static_cast<int>(q.size(1)), static_cast<int>(p.heads),

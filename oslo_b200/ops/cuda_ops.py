@@ -1138,12 +1138,17 @@ def moe_experts(h: Tensor, idx: Tensor, up: Tensor, down: Tensor, unit: str = "r
 
 
 # ---------------------------------------------------------------------------------------------------------------
-def _packed_heads(t: Tensor) -> Tensor:
-    """``[rows, heads, D]`` as the kernels of packed and paged sequences read it: contiguous D, 16-byte aligned heads inside their row."""
-    r, h, d = t.stride()
-    if d != 1 or r % 8 or h % 8 or t.data_ptr() % 16 or (h > r and t.size(0) > 1 and t.size(1) > 1) or (h <= 0 and t.size(1) > 1) or (r <= 0 and t.size(0) > 1):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+_OPS = {}
+
+
+def _op(name: str):
+    """An operator's only overload, looked up once: what a call of a few microseconds' work can save on the host."""
+    if _get_config().debug_sync:
+        return getattr(_ext(), name)
+    fn = _OPS.get(name)
+    if fn is None:
+        fn = _OPS[name] = getattr(load_ext(required=True), name).default
+    return fn
 
 
 def ragged_ok(q: Tensor, k: Tensor, v: Tensor) -> bool:
@@ -1153,8 +1158,7 @@ def ragged_ok(q: Tensor, k: Tensor, v: Tensor) -> bool:
 class _Ragged(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, key_offsets, scale, window):
-        q, k, v = _packed_heads(q), _packed_heads(k), _packed_heads(v)
-        o, lse = _ext().ragged_fwd(q, k, v, offsets, key_offsets, scale, window, True)
+        o, lse = _op("ragged_fwd")(q, k, v, offsets, key_offsets, scale, window, True)
         ctx.save_for_backward(q, k, v, o, lse, offsets, key_offsets)
         ctx.cfg = (scale, window)
         return o
@@ -1163,28 +1167,32 @@ class _Ragged(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, offsets, key_offsets = ctx.saved_tensors
-        dq, dk, dv = _ext().ragged_bwd(_packed_heads(do), q, k, v, o, lse, offsets, key_offsets, *ctx.cfg)
+        dq, dk, dv = _op("ragged_bwd")(do, q, k, v, o, lse, offsets, key_offsets, *ctx.cfg)
         return dq, dk, dv, None, None, None, None
 
 
 def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offsets: Tensor, window: Optional[int], scale: float) -> Tensor:
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Ragged.apply(q, k, v, offsets, key_offsets, float(scale), int(window or 0))
-    return _ext().ragged_fwd(_packed_heads(q), _packed_heads(k), _packed_heads(v), offsets, key_offsets, scale, window or 0, False)[0]
+    return _op("ragged_fwd")(q, k, v, offsets, key_offsets, scale, window or 0, False)[0]
+
+
+def _plain(t: Tensor) -> Tensor:
+    return t.detach() if t.requires_grad else t
 
 
 def paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale) -> None:
-    _ext().paged_append(_packed_heads(k.detach()), _packed_heads(v.detach()), k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)
+    _op("paged_append")(_plain(k), _plain(v), k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)
 
 
 def paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype):
     if dtype is None:
         dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
-    return _ext().paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype)
+    return _op("paged_read")(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype)
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, window, scale, k_scale, v_scale) -> Tensor:
-    return _ext().paged_attn(_packed_heads(q.detach()), k_pages, v_pages, page_table, lengths, scale, window or 0, k_scale, v_scale)
+    return _op("paged_attn")(_plain(q), k_pages, v_pages, page_table, lengths, scale, window or 0, k_scale, v_scale)
 
 
 def sample_ok(logits: Tensor) -> bool:
@@ -1193,12 +1201,9 @@ def sample_ok(logits: Tensor) -> bool:
 
 
 def sample_tokens(logits, uniform, temperature, top_k, top_p, min_p) -> Tensor:
-    x = logits.detach()
+    x = _plain(logits)
     if x.stride(1) != 1 and x.size(1) > 1:
         x = x.contiguous()
-    tensors, numbers = [], []
-    for value, default in ((temperature, 1.0), (top_k, 0), (top_p, 1.0), (min_p, 0.0)):
-        own = isinstance(value, Tensor)
-        tensors.append(value if own else None)
-        numbers.append(default if own else value)
-    return _ext().sample_tokens(x, uniform, *tensors, *numbers)
+    own = [v if isinstance(v, Tensor) else None for v in (temperature, top_k, top_p, min_p)]
+    numbers = [d if t is not None else v for t, v, d in zip(own, (temperature, top_k, top_p, min_p), (1.0, 0, 1.0, 0.0))]
+    return _op("sample_tokens")(x, uniform, *own, *numbers)

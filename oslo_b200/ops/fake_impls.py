@@ -348,7 +348,7 @@ def register() -> None:
 
     @reg("oslo_b200::ragged_fwd")
     def _(q, k, v, offsets, key_offsets, scale, window, with_lse):
-        return q.new_empty(q.shape), q.new_empty(q.shape[:2] if with_lse else (0,), dtype=torch.float32)
+        return q.new_empty(q.shape), q.new_empty((q.size(0) if with_lse else 0, q.size(1)), dtype=torch.float32)
 
     @reg("oslo_b200::ragged_bwd")
     def _(dout, q, k, v, o, lse, offsets, key_offsets, scale, window):

@@ -367,6 +367,20 @@ def selective_scan(x: Tensor, dt: Tensor, dt_bias: Tensor, a_log: Tensor, b: Ten
 
 # ---------------------------------------------------------------------------------------------------------------
 # Sequences of different lengths: packed behind one another, or in the pages of a shared pool.
+_CUDA_OPS = None
+
+
+def _kernels(x: Tensor):
+    """``cuda_ops`` where ``x`` must run on the kernels, else ``None``; looked up once, since these calls may be a few microseconds long."""
+    global _CUDA_OPS
+    if not x.is_cuda:
+        return None
+    if _CUDA_OPS is None and _k(x):
+        from . import cuda_ops
+        _CUDA_OPS = cuda_ops
+    return _CUDA_OPS
+
+
 def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offsets: Optional[Tensor] = None, window: Optional[int] = None,
                      scale: Optional[float] = None) -> Tensor:
     """Causal attention of packed sequences with grouped heads: ``q`` ``[T, heads, D]``, ``k`` and ``v`` ``[T_k, kv_heads, D]``.
@@ -379,10 +393,9 @@ def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
     sequence only)."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.size(-1))
-    if _k(q):
-        from . import cuda_ops
-        if cuda_ops.ragged_ok(q, k, v):
-            return cuda_ops.ragged_attention(q, k, v, offsets, offsets if key_offsets is None else key_offsets, window, scale)
+    kernels = _kernels(q)
+    if kernels is not None and kernels.ragged_ok(q, k, v):
+        return kernels.ragged_attention(q, k, v, offsets, offsets if key_offsets is None else key_offsets, window, scale)
     return ref.ragged_attention(q, k, v, offsets, key_offsets, window, scale)
 
 
@@ -395,9 +408,9 @@ def paged_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
     ``[B, columns]``) names a sequence's pages in order; ``lengths`` (int32 ``[B]``) counts its tokens, the new ones among them.
     Sequence ``b``'s new tokens are the rows ``offsets[b]`` to ``offsets[b + 1] - 1``, its last ones (``None``: one row per sequence).
     A sequence without a length, a position without a page and rows of no sequence are passed over. No gradients."""
-    if _k(k):
-        from . import cuda_ops
-        return cuda_ops.paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)
+    kernels = _kernels(k)
+    if kernels is not None:
+        return kernels.paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)
     return ref.paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)
 
 
@@ -406,9 +419,9 @@ def paged_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, offsets: Te
     """The keys and values ``[tokens, kv_heads, D]`` that a paged cache holds (see ``paged_append``), sequence behind sequence: the rows
     ``offsets[b]`` to ``offsets[b + 1] - 1`` are the first tokens of sequence ``b``, as ``ragged_attention`` takes them. ``dtype``: the
     result's type where the pools are 8-bit. Rows without a page give zeros."""
-    if _k(k_pages):
-        from . import cuda_ops
-        return cuda_ops.paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype)
+    kernels = _kernels(k_pages)
+    if kernels is not None:
+        return kernels.paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype)
     return ref.paged_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype)
 
 
@@ -419,9 +432,9 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     zeros; tokens without a page are passed over. No gradients."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.size(-1))
-    if _k(q):
-        from . import cuda_ops
-        return cuda_ops.paged_attention(q, k_pages, v_pages, page_table, lengths, window, scale, k_scale, v_scale)
+    kernels = _kernels(q)
+    if kernels is not None:
+        return kernels.paged_attention(q, k_pages, v_pages, page_table, lengths, window, scale, k_scale, v_scale)
     return ref.paged_attention(q, k_pages, v_pages, page_table, lengths, window, scale, k_scale, v_scale)
 
 
@@ -439,8 +452,7 @@ def sample_tokens(logits: Tensor, uniform: Tensor, temperature=1.0, top_k=0, top
             raise ValueError(f"sample_tokens: {name} must not be negative")
     if not logits.is_floating_point():
         raise ValueError("sample_tokens: logits must be floating-point numbers")
-    if _k(logits):
-        from . import cuda_ops
-        if cuda_ops.sample_ok(logits):
-            return cuda_ops.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
+    kernels = _kernels(logits)
+    if kernels is not None and kernels.sample_ok(logits):
+        return kernels.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
     return ref.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)

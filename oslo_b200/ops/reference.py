@@ -737,11 +737,13 @@ def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
 
 
 def quantise(x: Tensor) -> Tuple[Tensor, Tensor]:
-    """Vectors as e4m3 values and the fp32 number that multiplies them: largest magnitude over 448."""
+    """Vectors as e4m3 values and the fp32 number that multiplies them: largest magnitude over 448. Vectors that hold an infinity or no
+    number read back as no numbers, those too small for the number's reciprocal (10^-36) as zeros."""
     x = x.float()
     scale = x.abs().amax(-1) * torch.tensor(1.0 / FP8_MAX, dtype=torch.float32)     # one rounding on every device
-    scale = torch.where(torch.isfinite(scale), scale, float("nan"))
-    return (x / torch.where(scale == 0, 1.0, scale)[..., None]).to(torch.float8_e4m3fn), scale
+    by = torch.reciprocal(scale)
+    by = torch.where(torch.isfinite(by), by, 0.0)
+    return (x * by[..., None]).to(torch.float8_e4m3fn), torch.where(torch.isfinite(scale), scale, float("nan"))
 
 
 def _check_pages(op: str, k_pages, v_pages, page_table, k_scale, v_scale) -> None:
