@@ -90,8 +90,8 @@ std::tuple<Tensor, Tensor, Tensor> ragged_bwd(const Tensor& dout_, const Tensor&
     dq.zero_(); dk.zero_(); dv.zero_();
     return {dq, dk, dv};
   }
-  Tensor delta = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
-  check_rc(oslo_ragged_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), delta.data_ptr<float>(),
+  Tensor stats = at::empty({q.size(0), q.size(1), 2}, q.options().dtype(at::kFloat));
+  check_rc(oslo_ragged_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), stats.data_ptr<float>(),
                            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), off.data_ptr<int>(), koff.data_ptr<int>(), static_cast<int>(off.numel() - 1),
                            static_cast<int>(q.size(1)), static_cast<int>(k.size(1)), q.size(0), k.size(0), static_cast<int>(D), q.stride(0),
                            q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), o.stride(0), o.stride(1), dout.stride(0), dout.stride(1),

@@ -418,8 +418,8 @@ int oslo_ragged_fwd(const void* q, const void* k, const void* v, void* o, float*
                     int Hk, long long Tq, long long Tk, int D, long long q_sr, long long q_sh, long long k_sr, long long k_sh,
                     long long v_sr, long long v_sh, long long o_sr, long long o_sh, float scale, int window, int dtype, int* err_word,
                     cudaStream_t stream);
-// three launches (four where D > 128); delta: workspace [Tq, Hq]
-int oslo_ragged_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, float* delta, void* dq,
+// three launches (four where D > 128); stats: workspace [Tq, Hq, 2]
+int oslo_ragged_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, float* stats, void* dq,
                     void* dk, void* dv, const int* q_off, const int* k_off, int B, int Hq, int Hk, long long Tq, long long Tk, int D,
                     long long q_sr, long long q_sh, long long k_sr, long long k_sh, long long v_sr, long long v_sh, long long o_sr,
                     long long o_sh, long long g_sr, long long g_sh, long long dq_sr, long long dq_sh, long long dk_sr, long long dk_sh,

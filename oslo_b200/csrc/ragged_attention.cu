@@ -13,7 +13,9 @@
 //   dK, dV   rows = keys      S^T = K Q^T, dP^T = V dO^T   P^T, dS^T = P^T o (dP - delta)   dV += P^T dO, dK += dS^T Q
 //   dQ       rows = queries   S = Q K^T, dP = dO V^T       dS = P o (dP - delta)        dQ += dS K
 //
-// P and dS are rounded to the inputs' type for the second products (half a step, 2^-9 or 2^-11 of a weight); maxima, sums and all
+// P is rounded to the inputs' type for its products (half a step: 2^-9 of a weight, or 2^-12 in fp16), as the results are. dS, a difference,
+// goes into its products as two numbers of that type: rounded to one, dQ and dK were 1.5 (bf16) to 1.9 (fp16) times as far from the formula
+// as their own rounding puts them, now 1.1 to 1.4 times; it costs 5 % of the backward pass with heads of 128. Maxima, sums and all
 // accumulators are 32-bit.
 //
 // Not in the reference, which pads batches (oslo/models/gptj/modeling_gptj.py:151-191 is the attention of one).
@@ -30,7 +32,7 @@ struct RaggedParams {
   void* out; long long o_sr, o_sh;          // forward: O. backward: the gradient of this launch
   void* out2; long long o2_sr, o2_sh;       // dK beside dV
   float* lse;                               // [Tq, Hq], natural logarithm
-  const float* delta;                       // [Tq, Hq]
+  const float2* stats;                      // backward: [Tq, Hq] of -(log-sum-exp in log2 units) and -delta
   int* err;
 };
 
@@ -91,6 +93,69 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two at a time: a * k + b, and a sum
+__device__ __forceinline__ float2 fma2(float2 a, float k, float b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(k), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float k, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%6, %6};\n\tmov.b64 z, {%4, %5};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(k));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2v(float2 a, float2 b, float c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %6};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c));
+  return r;
+}
+// 2^x of two numbers up to 100 on the FMA pipe, to 2.6e-6 of its value: x = n + f with |f| <= 1/2 (n by adding 1.5 * 2^23), 2^f by a
+// polynomial of degree 4 with the least largest relative error (found by reweighted least squares), n into the exponent
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x.x = fmaxf(x.x, -125.f);
+  x.y = fmaxf(x.y, -125.f);
+  const float2 t = fma2(x, 1.f, 12582912.f), n = fma2(t, 1.f, -12582912.f), f = fma2v(n, make_float2(-1.f, -1.f), 0.f);
+  const float2 g = make_float2(x.x + f.x, x.y + f.y);
+  float2 e = fma2(g, 0.009570101698774808f, 0.05591786030272724f);
+  e = fma2v(e, g, 0.24024744833108522f);
+  e = fma2v(e, g, 0.6931218147397942f);
+  e = fma2v(e, g, 0.999999261444132f);
+  return make_float2(__uint_as_float(__float_as_uint(e.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(e.y) + (__float_as_uint(t.y) << 23)));
+}
+// a and b as 16-bit values and what those lack, as 16-bit values too: together 16 (bf16) or 22 (fp16) bits of them
+template <bool F16> __device__ __forceinline__ void split2(float2 a, uint32_t& hi, uint32_t& lo) {
+  float2 h;
+  if (F16) {
+    hi = fa_pack2(a.x, a.y, true);
+    h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  } else {                                          // cut off, not rounded: a byte permutation
+    const uint32_t x = __float_as_uint(a.x), y = __float_as_uint(a.y);
+    hi = __byte_perm(x, y, 0x7632);
+    h = make_float2(__uint_as_float(x & 0xffff0000u), __uint_as_float(y & 0xffff0000u));
+  }
+  a = fma2(h, -1.f, a);
+  lo = fa_pack2(a.x, a.y, F16);
+}
 __device__ __forceinline__ void ragged_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int head, int row) {
   tma_load_3d(dst, map, bar, col, head, row);
 }
@@ -138,22 +203,31 @@ __device__ __forceinline__ void ragged_store(uint32_t acc, int from, int to, boo
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // MT tiles of 128 rows per CTA. D <= 128: two, with a softmax warpgroup each (thread = row), so that the tensor core works for one tile
-// while the other's exponentials run; TMEM holds S (128 columns) and O (DP columns) of both, P overwrites S. D = 256: one tile, S of two
-// blocks of 64 keys. Warp 0: TMA, warp 1: MMA, warps 2-5 (and 6-9): softmax.
+// while the other's exponentials run. S of two blocks of 64 keys per tile: Q K^T of the next block runs under the softmax of this one (with
+// blocks of 128 keys TMEM holds one S a tile; its Q K^T then waited for P V: 350 us instead of 312 for 2 x 4096 tokens, 32/8 heads of
+// 128). P overwrites S. Warp 0: TMA; a warp a tile issues its products; then a warpgroup a tile for the softmax. A wait that is over at once
+// still takes 100 to 200 cycles and a commit not much less, so an issuer has two of each a block: K of the next block and V of this one
+// share a stage (with one warp for both tiles and five waits and commits a tile: 449 us).
 template <int DP> struct RaggedFwd {
-  static constexpr int MT = DP <= 128 ? 2 : 1, BN = DP <= 128 ? 128 : 64;
-  static constexpr int THREADS = 64 + 128 * MT, ROWS = 128 * MT;
+  static constexpr int MT = DP <= 128 ? 2 : 1, BN = 64;
+  static constexpr int FIRST = 1 + MT, THREADS = 32 * (FIRST + 4 * MT), ROWS = 128 * MT;      // FIRST: the first softmax warp
   static constexpr int DC = DP / 64;
+  // of 8 pairs of exponentials, those that the FMA pipe computes: 16 a clock come from the special function unit, half of a block's time.
+  // 0, 1, 2, 3 of 8: 315, 305, 304, 305 us for heads of 128, 285, 277, 275, 276 for 64, 521, 525, 535, 539 for 256 (its products wait for
+  // one tile's softmax only; the longer chain of the polynomial shows)
+  static constexpr int FMA_EXP = DP <= 128 ? 2 : 0;
   static constexpr uint32_t Q_SUB = 128 * 128, Q_TILE = DC * Q_SUB, KV_SUB = BN * 128, KV_TILE = DC * KV_SUB;
-  static constexpr int STAGES = DP == 64 ? 3 : 2;
-  static constexpr uint32_t S_COL = 0, O_COL = 256;                // DP = 256: S 0..127, O 256..511
-  static constexpr uint32_t TILES = MT * Q_TILE + 2 * STAGES * KV_TILE;
-  static constexpr int B_Q = 0, B_KF = 1, B_KE = B_KF + STAGES, B_VF = B_KE + STAGES, B_VE = B_VF + STAGES, B_S = B_VE + STAGES,
-                       B_P = B_S + 2, B_O = B_P + 2, B_PV = B_O + 2, BARS = B_PV + 1;
+  static constexpr int STAGES = DP == 256 ? 2 : (DP == 128 ? 4 : 6);       // of K of block j + 1 and V of block j
+  static constexpr uint32_t S_COL = 0, O_COL = 256;                // S: tile i, buffer b at (2 i + b) BN
+  static_assert(2 * MT * BN <= 256 && MT * DP <= 256, "TMEM budget");
+  static constexpr uint32_t TILES = MT * Q_TILE + (1 + 2 * STAGES) * KV_TILE;
+  static constexpr int B_Q = 0, B_F = 1, B_E = B_F + STAGES, B_S = B_E + STAGES, B_P = B_S + 4, B_O = B_P + 4, B_W = B_O + 2,
+                       BARS = B_W + 1;                             // B_Q: Q and the first K; B_S, B_P: 2 tile + buffer; B_W: rows wiped
   static constexpr uint32_t SMEM = TILES + BARS * 8 + 64 + 1024;
 };
 
-template <int DP>
+// F16: the inputs are fp16 (a branch at every packed pair otherwise)
+template <int DP, bool F16>
 __global__ void __launch_bounds__(RaggedFwd<DP>::THREADS, 1)
 ragged_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const RaggedParams p) {
@@ -161,7 +235,9 @@ ragged_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   constexpr int BN = F::BN, MT = F::MT, DC = F::DC, ST = F::STAGES;
   extern __shared__ uint8_t ragged_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ragged_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t q_s = smem_u32(smem), k_s = q_s + MT * F::Q_TILE, v_s = k_s + ST * F::KV_TILE;
+  const uint32_t q_s = smem_u32(smem), kv_s = q_s + MT * F::Q_TILE;       // K of block 0, then the stages
+  auto k_at = [&](int j) { return j == 0 ? kv_s : kv_s + (1 + 2 * ((j - 1) % ST)) * F::KV_TILE; };
+  auto v_at = [&](int j) { return kv_s + (2 + 2 * (j % ST)) * F::KV_TILE; };
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::TILES);
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
@@ -176,7 +252,9 @@ ragged_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     if (lane == 0) *found = t;
   }
   if (threadIdx.x == 32) {
-    for (int i = 0; i < F::BARS; ++i) mbar_init(bar(i), i >= F::B_P && i < F::B_P + 2 ? 4 : 1);
+    // four softmax warps hand over a P; every tile's issuer gives a stage back
+    for (int i = 0; i < F::BARS; ++i)
+      mbar_init(bar(i), i >= F::B_P && i < F::B_P + 4 ? 4 : (i >= F::B_E && i < F::B_S ? MT : 1));
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -206,205 +284,187 @@ ragged_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       n[i] = hi > lo ? (hi - lo + BN - 1) / BN : 0;
     }
   }
-  const int blocks = max(n[0], n[1]);
+  const int blocks = max(n[0], n[1]), tail = t.nk - (lo + (blocks - 1) * BN);      // tail: keys of the sequence in the last block
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
+    int ok = blocks > 0;
     if (lane == 0 && blocks > 0) {
       tma_prefetch_desc(&tq); tma_prefetch_desc(&tk); tma_prefetch_desc(&tv);
-      mbar_expect_tx(bar(F::B_Q), MT * F::Q_TILE);
+      mbar_expect_tx(bar(F::B_Q), MT * F::Q_TILE + F::KV_TILE);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int c = 0; c < DC; ++c)
           ragged_load(q_s + i * F::Q_TILE + c * F::Q_SUB, &tq, bar(F::B_Q), c * 64, h0, t.q0 + ((t.first + i * 128) >> p.pack_log));
-      bool ok = true;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) ragged_load(kv_s + c * F::KV_SUB, &tk, bar(F::B_Q), c * 64, hk, t.k0 + lo);
       for (int j = 0; j < blocks && ok; ++j) {
-        const int st = j % ST;
-        const uint32_t ph = (j / ST) & 1;
-        const int row = t.k0 + lo + j * BN;
-        ok = mbar_wait(bar(F::B_KE + st), ph ^ 1, abort_flag, p.err, ERR_WAIT_EMPTY);
+        const int st = j % ST, row = t.k0 + lo + j * BN;
+        ok = mbar_wait(bar(F::B_E + st), ((j / ST) & 1) ^ 1, abort_flag, p.err, ERR_WAIT_EMPTY);
         if (!ok) break;
-        mbar_expect_tx(bar(F::B_KF + st), F::KV_TILE);
+        mbar_expect_tx(bar(F::B_F + st), j + 1 < blocks ? 2 * F::KV_TILE : F::KV_TILE);
+        if (j + 1 < blocks) {
 #pragma unroll
-        for (int c = 0; c < DC; ++c) ragged_load(k_s + st * F::KV_TILE + c * F::KV_SUB, &tk, bar(F::B_KF + st), c * 64, hk, row);
-        ok = mbar_wait(bar(F::B_VE + st), ph ^ 1, abort_flag, p.err, ERR_WAIT_EMPTY);
-        if (!ok) break;
-        mbar_expect_tx(bar(F::B_VF + st), F::KV_TILE);
+          for (int c = 0; c < DC; ++c) ragged_load(k_at(j + 1) + c * F::KV_SUB, &tk, bar(F::B_F + st), c * 64, hk, row + BN);
+        }
 #pragma unroll
-        for (int c = 0; c < DC; ++c) ragged_load(v_s + st * F::KV_TILE + c * F::KV_SUB, &tv, bar(F::B_VF + st), c * 64, hk, row);
+        for (int c = 0; c < DC; ++c) ragged_load(v_at(j) + c * F::KV_SUB, &tv, bar(F::B_F + st), c * 64, hk, row);
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer: the whole warp runs the loops, one lane issues
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    if (ok && tail < BN) {                  // the last block's values of other sequences
+      const int j = blocks - 1;
+      if (mbar_wait_warp(bar(F::B_F + j % ST), (j / ST) & 1, abort_flag, p.err, ERR_WAIT_FULL)) {
+        ragged_wipe(v_at(j), tail, BN, DC);
+        if (lane == 0) mbar_arrive(bar(F::B_W));
+      }
+    }
+  } else if (warp <= MT) {
+    // ------------------------------------------------------------------ MMA issuer of a tile: the whole warp runs the loop, so that
+    // addresses and descriptors are uniform; one lane issues
+    const int i = warp - 1;
     if (blocks > 0) {
-      const int fmt = p.fp16 ? 0 : 1;
+      constexpr int fmt = F16 ? 0 : 1;
       const uint32_t idesc_qk = make_idesc_f16(128, BN, fmt, 0, 0), idesc_pv = make_idesc_f16(128, DP, fmt, 0, 1);
+      const uint64_t desc_k = make_smem_desc(0, 16, 1024), desc_v = make_smem_desc(0, F::KV_SUB, 1024);      // plus (address >> 4)
       const bool issuer = elect_one();
-      bool ok = mbar_wait_warp(bar(F::B_Q), 0, abort_flag, p.err, ERR_WAIT_FULL);
-      // S of tile i and block j: TMEM buffer i (two tiles) or j & 1 (one tile)
-      auto qk = [&](int i, int j) -> bool {
-        const int st = j % ST, buf = MT == 2 ? i : j & 1;
-        if (!mbar_wait_warp(bar(F::B_KF + st), (j / ST) & 1, abort_flag, p.err, ERR_WAIT_FULL)) return false;
+      auto wait = [&](int b, uint32_t parity) { return mbar_wait_warp(bar(b), parity, abort_flag, p.err, ERR_WAIT_FULL); };
+      auto qk = [&](int j) {
+        const uint64_t da = desc_k + ((q_s + i * F::Q_TILE) >> 4), db = desc_k + (k_at(j) >> 4);
+        const uint32_t dst = tmem + F::S_COL + (2 * i + (j & 1)) * BN;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+          umma_f16(dst, da + (((kk >> 2) * F::Q_SUB + (kk & 3) * 32) >> 4), db + (((kk >> 2) * F::KV_SUB + (kk & 3) * 32) >> 4), idesc_qk, kk != 0);
+      };
+      bool ok = wait(F::B_Q, 0);
+      tc_fence_after();
+      if (ok && n[i] > 0 && issuer) {
+        qk(0);
+        umma_commit(bar(F::B_S + 2 * i));
+      }
+      __syncwarp();
+      for (int j = 0; j < n[i]; ++j) {
+        const int st = j % ST, buf = 2 * i + (j & 1);
+        ok = wait(F::B_F + st, (j / ST) & 1);
+        if (!ok) break;
         tc_fence_after();
         if (issuer) {
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
-            const uint64_t da = make_smem_desc(q_s + i * F::Q_TILE + (kk >> 2) * F::Q_SUB + (kk & 3) * 32, 16, 1024);
-            const uint64_t db = make_smem_desc(k_s + st * F::KV_TILE + (kk >> 2) * F::KV_SUB + (kk & 3) * 32, 16, 1024);
-            umma_f16(tmem + F::S_COL + buf * BN, da, db, idesc_qk, kk != 0);
-          }
-          umma_commit(bar(F::B_S + buf));
+          // S of block j + 1 takes the place of P of block j - 1, whose product was issued before: those of one thread run in order.
+          // The commit, also without a block j + 1, says that O holds block j - 1.
+          if (j + 1 < n[i]) qk(j + 1);
+          umma_commit(bar(F::B_S + (buf ^ 1)));
         }
         __syncwarp();
-        return true;
-      };
-      auto pv = [&](int i, int j) -> bool {
-        const int st = j % ST, buf = MT == 2 ? i : j & 1;
-        const uint32_t ph = MT == 2 ? j & 1 : (j >> 1) & 1;
-        if (!mbar_wait_warp(bar(F::B_VF + st), (j / ST) & 1, abort_flag, p.err, ERR_WAIT_FULL)) return false;
-        const int left = t.nk - (lo + j * BN);
-        if (left < BN && (MT == 1 || i == (j < n[0] ? 0 : 1))) ragged_wipe(v_s + st * F::KV_TILE, left, BN, DC);   // once per block
-        if (!mbar_wait_warp(bar(F::B_P + buf), ph, abort_flag, p.err, ERR_WAIT_FULL)) return false;
+        ok = (j + 1 < blocks || tail >= BN || wait(F::B_W, 0)) && wait(F::B_P + buf, (j >> 1) & 1);
+        if (!ok) break;
         tc_fence_after();
         if (issuer) {
+          const uint64_t db = desc_v + (v_at(j) >> 4);
+          const uint32_t src = tmem + F::S_COL + buf * BN;
 #pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks) {
-            const uint64_t db = make_smem_desc(v_s + st * F::KV_TILE + ks * 2048, F::KV_SUB, 1024);
-            umma_f16_ts(tmem + F::O_COL + i * DP, tmem + F::S_COL + buf * BN + ks * 8, db, idesc_pv, (j | ks) != 0);
-          }
-          if (MT == 1) umma_commit(bar(F::B_PV));
+          for (int ks = 0; ks < BN / 16; ++ks) umma_f16_ts(tmem + F::O_COL + i * DP, src + ks * 8, db + ks * 128, idesc_pv, (j | ks) != 0);
+          umma_commit(bar(F::B_E + st));
           if (j + 1 == n[i]) umma_commit(bar(F::B_O + i));
         }
         __syncwarp();
-        return true;
-      };
-      auto release = [&](int b) {
-        if (issuer) umma_commit(bar(b));
-        __syncwarp();
-      };
-      if (MT == 2) {
-        for (int i = 0; i < 2 && ok; ++i)
-          if (n[i] > 0) ok = qk(i, 0);
-        if (ok) release(F::B_KE);
-        for (int j = 0; j < blocks && ok; ++j) {
-          for (int i = 0; i < 2 && ok; ++i) {
-            if (j >= n[i]) continue;
-            ok = pv(i, j);
-            if (ok && j + 1 < n[i]) ok = qk(i, j + 1);              // S of block j is consumed: products of one thread run in order
-          }
-          if (!ok) break;
-          release(F::B_VE + j % ST);
-          if (j + 1 < blocks) release(F::B_KE + (j + 1) % ST);
-        }
-      } else {
-        if (ok) ok = qk(0, 0);
-        if (ok) release(F::B_KE);
-        for (int j = 0; j < blocks && ok; ++j) {
-          if (j + 1 < blocks) {
-            ok = qk(0, j + 1);
-            if (!ok) break;
-            release(F::B_KE + (j + 1) % ST);
-          }
-          ok = pv(0, j);
-          if (ok) release(F::B_VE + j % ST);
-        }
+      }
+      // blocks that only the other tile needs: given back as they come (not before: an arrival belongs to its own round)
+      for (int j = n[i]; j < blocks && ok; ++j) {
+        ok = wait(F::B_F + j % ST, (j / ST) & 1);
+        if (ok && issuer) mbar_arrive(bar(F::B_E + j % ST));
       }
     }
   } else {
     // ------------------------------------------------------------------ softmax: thread = row
-    const int i = MT == 2 ? (warp - 2) >> 2 : 0, quad = warp & 3;
+    const int i = (warp - F::FIRST) >> 2, quad = warp & 3;
     const int r = t.first + i * 128 + quad * 32 + lane, tok = r >> p.pack_log, head = h0 + (r & (p.pack - 1));
     const bool live = r < rows;
     const uint32_t lane_at = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t o_at = lane_at + F::O_COL + i * DP;
     const float sc = p.scale * FA_LOG2E;
-    const bool fp16 = p.fp16 != 0;
+    constexpr bool fp16 = F16;
     const int last = min(t.nk - 1, tok + offset), first = p.window > 0 ? tok + offset - p.window + 1 : 0;
     const int first_tok = (t.first + i * 128) >> p.pack_log, last_tok = (t.first + i * 128 + 127) >> p.pack_log;
     float m = -CUDART_INF_F, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < n[i] && ok; ++j) {
-      const int buf = MT == 2 ? i : j & 1, n0 = lo + j * BN;
-      ok = mbar_wait_warp(bar(F::B_S + buf), MT == 2 ? j & 1 : (j >> 1) & 1, abort_flag, p.err, ERR_WAIT_TMEM_FULL);
+    for (int j = 0; j < n[i]; ++j) {
+      const int buf = 2 * i + (j & 1), n0 = lo + j * BN;
+      ok = mbar_wait_warp(bar(F::B_S + buf), (j >> 1) & 1, abort_flag, p.err, ERR_WAIT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
       const uint32_t s_at = lane_at + F::S_COL + buf * BN;
-      float s[BN];
+      uint32_t x[BN / 32][32];
 #pragma unroll
-      for (int c0 = 0; c0 < BN; c0 += 32) {
-        uint32_t x[32];
-        tmem_ld_32x32(s_at + c0, x);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; ++c) s[c0 + c] = __uint_as_float(x[c]);
-      }
+      for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32(s_at + c * 32, x[c]);
+      tmem_wait_ld();
+      auto s = [&](int c) -> float { return __uint_as_float(x[c >> 5][c & 31]); };
       // only blocks that reach past the diagonal, the window's edge or the keys' end of some row
       if (n0 + BN > min(t.nk, first_tok + offset + 1) || (p.window > 0 && n0 <= last_tok + offset - p.window)) {
         auto below = [](int k) { return k <= 0 ? 0u : (k >= 32 ? 0xffffffffu : (1u << k) - 1u); };
 #pragma unroll
-        for (int c0 = 0; c0 < BN; c0 += 32) {
-          const uint32_t vis = below(last - (n0 + c0) + 1) & ~below(first - (n0 + c0));
+        for (int c = 0; c < BN / 32; ++c) {
+          const uint32_t vis = below(last - (n0 + c * 32) + 1) & ~below(first - (n0 + c * 32));
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!((vis >> c) & 1u)) s[c0 + c] = -CUDART_INF_F;
+          for (int u = 0; u < 32; ++u)
+            if (!((vis >> u) & 1u)) x[c][u] = 0xff800000u;
         }
       }
-      float mx4[4] = {s[0], s[1], s[2], s[3]};
+      float mx4[4] = {s(0), s(1), s(2), s(3)};
 #pragma unroll
-      for (int c = 4; c < BN; c += 4) {
+      for (int c = 4; c + 8 <= BN; c += 8) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(mx4[u], s[c + u]);
+        for (int u = 0; u < 4; ++u) mx4[u] = max3(mx4[u], s(c + u), s(c + 4 + u));
       }
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc, m_new = fmaxf(m, mx);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(mx4[u], s(BN - 4 + u));
+      const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * sc, m_new = fmaxf(m, mx);
       // O is multiplied only when a row of this warp has outgrown its reference by 2^8
-      const bool rescale = __any_sync(0xffffffffu, j == 0 || m_new - m > 8.f);
-      float factor = 1.f;
-      if (rescale) {
-        factor = m == -CUDART_INF_F ? 0.f : exp2f(m - m_new);
+      if (__any_sync(0xffffffffu, j == 0 || m_new - m > 8.f)) {
+        const float factor = m == -CUDART_INF_F ? 0.f : exp2f(m - m_new);
         m = m_new;
         l *= factor;
-      }
-      const float base = m == -CUDART_INF_F ? 0.f : -m;
-      float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < BN; c += 4) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          s[c + u] = exp2f(fmaf(s[c + u], sc, base));
-          sum4[u] += s[c + u];
-        }
-      }
-      l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-      if (rescale && j > 0) {
-        // two tiles: P V of block j - 1 ended before S of block j; one tile: it is waited for
-        if (MT == 1) {
-          ok = mbar_wait_warp(bar(F::B_PV), (j - 1) & 1, abort_flag, p.err, ERR_WAIT_TMEM_FULL);
+        if (j > 0) {
+          // O holds block j - 1 as soon as S of block j + 1 is there
+          ok = mbar_wait_warp(bar(F::B_S + (buf ^ 1)), ((j + 1) >> 1) & 1, abort_flag, p.err, ERR_WAIT_TMEM_FULL);
           if (!ok) break;
           tc_fence_after();
-        }
 #pragma unroll 1
-        for (int c0 = 0; c0 < DP; c0 += 32) {
-          uint32_t x[32];
-          tmem_ld_32x32(o_at + c0, x);
-          tmem_wait_ld();
+          for (int c0 = 0; c0 < DP; c0 += 32) {
+            uint32_t y[32];
+            tmem_ld_32x32(o_at + c0, y);
+            tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * factor);
-          tmem_st_32x32(o_at + c0, x);
+            for (int c = 0; c < 32; ++c) y[c] = __float_as_uint(__uint_as_float(y[c]) * factor);
+            tmem_st_32x32(o_at + c0, y);
+          }
+          tmem_wait_st();
         }
-        tmem_wait_st();
       }
+      const float base = m == -CUDART_INF_F ? 0.f : -m;
+      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c0 = 0; c0 < BN / 2; c0 += 32) {
-        uint32_t x[32];
+      for (int c = 0; c < BN / 32; ++c) {
+        uint32_t w[16];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) x[c] = fa_pack2(s[2 * (c0 + c)], s[2 * (c0 + c) + 1], fp16);
-        tmem_st_32x32(s_at + c0, x);
+        for (int u = 0; u < 16; ++u) {
+          float2 e = fma2(make_float2(__uint_as_float(x[c][2 * u]), __uint_as_float(x[c][2 * u + 1])), sc, base);
+          if (u % 8 < F::FMA_EXP) {
+            e = exp2_fma(e);
+          } else {
+            e.x = exp2f(e.x);
+            e.y = exp2f(e.y);
+          }
+          sum2[u & 1] = add2(sum2[u & 1], e);
+          w[u] = fa_pack2(e.x, e.y, fp16);
+        }
+        tmem_st_32x16(s_at + c * 16, w);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(F::B_P + buf));
+      l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
     }
     if (ok && n[i] > 0) {
       ok = mbar_wait_warp(bar(F::B_O + i), 0, abort_flag, p.err, ERR_WAIT_TMEM_FULL);
@@ -431,10 +491,11 @@ ragged_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------------------------------------------- backward
-// delta[t, h] = sum_d dO O in 32 bits; DP / 8 lanes a row. Bound by reading both.
+// What the other kernels need of a query row: its log-sum-exp in log2 units and delta[t, h] = sum_d dO O in 32 bits, negative, side by side; DP / 8
+// lanes a row. Bound by reading both.
 template <typename T, int LPR>
-__global__ void __launch_bounds__(256) ragged_delta_kernel(const T* __restrict__ o, const T* __restrict__ g, float* __restrict__ delta,
-                                                           long long rows, int H, int D, long long o_sr, long long o_sh, long long g_sr,
+__global__ void __launch_bounds__(256) ragged_delta_kernel(const T* __restrict__ o, const T* __restrict__ g, const float* __restrict__ lse,
+                                                           float2* __restrict__ stats, long long rows, int H, int D, long long o_sr, long long o_sh, long long g_sr,
                                                            long long g_sh) {
   const long long row = static_cast<long long>(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR;
   const int d = threadIdx.x % LPR * 8;
@@ -458,7 +519,7 @@ __global__ void __launch_bounds__(256) ragged_delta_kernel(const T* __restrict__
   }
 #pragma unroll
   for (int s = LPR / 2; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
-  if (row < rows && d == 0) delta[row] = acc;
+  if (row < rows && d == 0) stats[row] = make_float2(-lse[row] * FA_LOG2E, -acc);
 }
 
 enum : int { RB_DKV = 0, RB_DV = 1, RB_DK = 2, RB_DQ = 3 };
@@ -468,20 +529,23 @@ enum : int { RB_DKV = 0, RB_DV = 1, RB_DK = 2, RB_DQ = 3 };
 // accumulators fill TMEM alone. r1, s1: what S is made of; r2, s2: what dP (and dV) is made of.
 template <int DP, int MODE> struct RaggedBwd {
   static constexpr bool KEY_ROWS = MODE != RB_DQ, DPROD = MODE != RB_DV;        // DPROD: dP is needed
-  static constexpr int BN = 64, THREADS = 64 + 256, DC = DP / 64;
+  static constexpr int BN = 64, DC = DP / 64, THREADS = 64 + 256 + (KEY_ROWS ? 32 : 0), NST = DP == 256 ? 2 : 4;    // NST: blocks of statistics
   static constexpr uint32_t R_SUB = 128 * 128, R_TILE = DC * R_SUB, C_SUB = BN * 128, C_TILE = DC * C_SUB;
   static constexpr int NRES = DPROD ? 2 : 1;
-  static constexpr int S1 = DP == 256 ? 2 : 3, S2 = DP == 256 ? (MODE == RB_DV ? 2 : 1) : (MODE == RB_DQ ? 2 : 3);
-  static constexpr uint32_t STATS = KEY_ROWS ? 2 * 2 * BN * 4 : 0;
+  // a copy takes longer than a block's products: as many blocks ahead as there is room for. JOINT: both operands of a block share a stage,
+  // which saves the issuer waits and commits (100 to 200 cycles each)
+  static constexpr bool JOINT = DP < 256;
+  static constexpr int S1 = DP == 256 ? 2 : (DP == 128 ? 4 : 6), S2 = DP == 256 ? (MODE == RB_DV ? 2 : 1) : S1;
+  static constexpr uint32_t STATS = KEY_ROWS ? NST * BN * 8 : 0;
   static constexpr uint32_t TILES = NRES * R_TILE + (S1 + S2) * C_TILE;
   static constexpr uint32_t S_COL = 0, DP_COL = 2 * BN, ACC = 4 * BN, ACC2 = ACC + DP;      // ACC2: dK beside dV
   static_assert((MODE == RB_DKV ? ACC2 : ACC) + DP <= 512, "TMEM budget");
   static constexpr int B_R = 0, B_1F = 1, B_1E = B_1F + S1, B_2F = B_1E + S1, B_2E = B_2F + S2, B_SP = B_2E + S2, B_TR = B_SP + 2,
-                       B_ST = B_TR + 2, B_ACC = B_ST + 2, BARS = B_ACC + 1;
+                       B_ST = B_TR + 2, B_SE = B_ST + NST, B_ACC = B_SE + NST, BARS = B_ACC + 1;
   static constexpr uint32_t SMEM = TILES + STATS + BARS * 8 + 64 + 1024;
 };
 
-template <int DP, int MODE>
+template <int DP, int MODE, bool F16>
 __global__ void __launch_bounds__(RaggedBwd<DP, MODE>::THREADS, 1)
 ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant__ CUtensorMap tr2, const __grid_constant__ CUtensorMap ts1,
                   const __grid_constant__ CUtensorMap ts2, const RaggedParams p) {
@@ -491,7 +555,7 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   extern __shared__ uint8_t ragged_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ragged_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t r1_s = smem_u32(smem), r2_s = r1_s + F::R_TILE, s1_s = r1_s + F::NRES * F::R_TILE, s2_s = s1_s + F::S1 * F::C_TILE;
-  float* stats = reinterpret_cast<float*>(smem + F::TILES);        // [2 blocks][lse in log2 units, delta][BN]
+  float2* stats = reinterpret_cast<float2*>(smem + F::TILES);      // [NST blocks][BN]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::TILES + F::STATS);
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
@@ -506,7 +570,7 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     if (lane == 0) *found = t;
   }
   if (threadIdx.x == 32) {
-    for (int i = 0; i < F::BARS; ++i) mbar_init(bar(i), i >= F::B_TR && i < F::B_TR + 2 ? 8 : 1);
+    for (int i = 0; i < F::BARS; ++i) mbar_init(bar(i), (i >= F::B_TR && i < F::B_TR + 2) || (i >= F::B_SE && i < F::B_SE + F::NST) ? 8 : 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -541,86 +605,101 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   auto heads_of = [&](int j) { return hk * group + (KEY_ROWS ? j / per : sub0) * p.pack; };
 
   if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer, statistics of the columns
-    if (blocks > 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0 && blocks > 0) {
       const int row = KEY_ROWS ? t.k0 + t.first : t.q0 + (t.first >> p.pack_log), rh = KEY_ROWS ? hk : heads_of(0);
-      if (lane == 0) {
-        tma_prefetch_desc(&tr1); tma_prefetch_desc(&tr2); tma_prefetch_desc(&ts1); tma_prefetch_desc(&ts2);
-        mbar_expect_tx(bar(F::B_R), F::NRES * F::R_TILE);
+      tma_prefetch_desc(&tr1); tma_prefetch_desc(&tr2); tma_prefetch_desc(&ts1); tma_prefetch_desc(&ts2);
+      mbar_expect_tx(bar(F::B_R), F::NRES * F::R_TILE);
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          ragged_load(r1_s + c * F::R_SUB, &tr1, bar(F::B_R), c * 64, rh, row);
-          if (F::DPROD) ragged_load(r2_s + c * F::R_SUB, &tr2, bar(F::B_R), c * 64, rh, row);
-        }
+      for (int c = 0; c < DC; ++c) {
+        ragged_load(r1_s + c * F::R_SUB, &tr1, bar(F::B_R), c * 64, rh, row);
+        if (F::DPROD) ragged_load(r2_s + c * F::R_SUB, &tr2, bar(F::B_R), c * 64, rh, row);
       }
-      for (int j = 0; j < blocks; ++j) {
+      bool ok = true;
+      for (int j = 0; j < blocks && ok; ++j) {
         const int c0 = column(j), ch = KEY_ROWS ? heads_of(j) : hk, cr = KEY_ROWS ? t.q0 + (c0 >> p.pack_log) : t.k0 + c0;
         const int st1 = j % F::S1, st2 = j % F::S2;
-        int ok = 1;
-        if (lane == 0) {
-          auto load = [&](const CUtensorMap* map, uint32_t dst, int full, int empty, uint32_t ph) -> bool {
-            if (!mbar_wait(bar(empty), ph ^ 1, abort_flag, p.err, ERR_WAIT_EMPTY)) return false;
-            mbar_expect_tx(bar(full), F::C_TILE);
+        auto load = [&](const CUtensorMap* map, uint32_t dst, int full, int empty, uint32_t ph) -> bool {
+          if (!mbar_wait(bar(empty), ph ^ 1, abort_flag, p.err, ERR_WAIT_EMPTY)) return false;
+          mbar_expect_tx(bar(full), F::C_TILE);
 #pragma unroll
-            for (int c = 0; c < DC; ++c) ragged_load(dst + c * F::C_SUB, map, bar(full), c * 64, ch, cr);
-            return true;
-          };
-          ok = load(&ts2, s2_s + st2 * F::C_TILE, F::B_2F + st2, F::B_2E + st2, (j / F::S2) & 1) &&
-               load(&ts1, s1_s + st1 * F::C_TILE, F::B_1F + st1, F::B_1E + st1, (j / F::S1) & 1) &&
-               // the statistics' buffer was last read by the transform of block j - 2
-               (!KEY_ROWS || mbar_wait(bar(F::B_TR + (j & 1)), ((j >> 1) & 1) ^ 1, abort_flag, p.err, ERR_WAIT_TMEM_EMPTY));
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
-        if (KEY_ROWS) {
-          float* sb = stats + (j & 1) * 2 * BN;
-          for (int i = lane; i < BN; i += 32) {
-            const int c = c0 + i;
-            float l2 = 0.f, dl = 0.f;
-            if (c < rows) {
-              const long long at = static_cast<long long>(t.q0 + (c >> p.pack_log)) * p.Hq + ch + (c & (p.pack - 1));
-              l2 = p.lse[at] * FA_LOG2E;
-              if (F::DPROD) dl = p.delta[at];
-            }
-            sb[i] = l2;
-            sb[BN + i] = dl;
+          for (int c = 0; c < DC; ++c) ragged_load(dst + c * F::C_SUB, map, bar(full), c * 64, ch, cr);
+          return true;
+        };
+        if (F::JOINT) {
+          ok = mbar_wait(bar(F::B_1E + st1), ((j / F::S1) & 1) ^ 1, abort_flag, p.err, ERR_WAIT_EMPTY);
+          if (!ok) break;
+          mbar_expect_tx(bar(F::B_1F + st1), 2 * F::C_TILE);
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            ragged_load(s2_s + st1 * F::C_TILE + c * F::C_SUB, &ts2, bar(F::B_1F + st1), c * 64, ch, cr);
+            ragged_load(s1_s + st1 * F::C_TILE + c * F::C_SUB, &ts1, bar(F::B_1F + st1), c * 64, ch, cr);
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(F::B_ST + (j & 1)));
+        } else {
+          ok = load(&ts2, s2_s + st2 * F::C_TILE, F::B_2F + st2, F::B_2E + st2, (j / F::S2) & 1) &&
+               load(&ts1, s1_s + st1 * F::C_TILE, F::B_1F + st1, F::B_1E + st1, (j / F::S1) & 1);
         }
       }
+    }
+  } else if (KEY_ROWS && warp == 10) {
+    // ------------------------------------------------------------------ statistics of the columns, two a lane
+    auto fetch = [&](int j, float2 (&v)[2]) {
+      const int c0 = column(j), ch = heads_of(j);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int c = c0 + lane * 2 + u;
+        v[u] = c < rows ? p.stats[static_cast<long long>(t.q0 + (c >> p.pack_log)) * p.Hq + ch + (c & (p.pack - 1))] : make_float2(0.f, 0.f);
+      }
+    };
+    float2 now[2], next[2];
+    if (blocks > 0) fetch(0, now);
+    for (int j = 0; j < blocks; ++j) {
+      if (j + 1 < blocks) fetch(j + 1, next);
+      const int st = j % F::NST;
+      if (!mbar_wait_warp(bar(F::B_SE + st), ((j / F::NST) & 1) ^ 1, abort_flag, p.err, ERR_WAIT_EMPTY)) break;
+      *reinterpret_cast<float4*>(stats + st * BN + lane * 2) = make_float4(now[0].x, now[1].x, now[0].y, now[1].y);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(F::B_ST + st));
+      now[0] = next[0];
+      now[1] = next[1];
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer: the whole warp runs the loops, one lane issues
     if (blocks > 0) {
-      const int fmt = p.fp16 ? 0 : 1;
+      constexpr int fmt = F16 ? 0 : 1;
       const uint32_t idesc_1 = make_idesc_f16(128, BN, fmt, 0, 0), idesc_2 = make_idesc_f16(128, DP, fmt, 0, 1);
+      const uint64_t desc_1 = make_smem_desc(0, 16, 1024), desc_2 = make_smem_desc(0, F::C_SUB, 1024);        // plus (address >> 4)
       const bool issuer = elect_one();
-      bool ok = mbar_wait_warp(bar(F::B_R), 0, abort_flag, p.err, ERR_WAIT_FULL);
+      auto wait = [&](int b, uint32_t parity) { return mbar_wait_warp(bar(b), parity, abort_flag, p.err, ERR_WAIT_FULL); };
       auto product = [&](uint32_t dst, uint32_t res, uint32_t tile) {
+        const uint64_t da = desc_1 + (res >> 4), db = desc_1 + (tile >> 4);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t da = make_smem_desc(res + (kk >> 2) * F::R_SUB + (kk & 3) * 32, 16, 1024);
-          const uint64_t db = make_smem_desc(tile + (kk >> 2) * F::C_SUB + (kk & 3) * 32, 16, 1024);
-          umma_f16(dst, da, db, idesc_1, kk != 0);
-        }
+        for (int kk = 0; kk < DP / 16; ++kk)
+          umma_f16(dst, da + (((kk >> 2) * F::R_SUB + (kk & 3) * 32) >> 4), db + (((kk >> 2) * F::C_SUB + (kk & 3) * 32) >> 4), idesc_1, kk != 0);
       };
+      // 16 columns a step; each half of the 64 columns has its packed values at its own first columns
+      auto second = [&](uint32_t acc, uint32_t src, uint32_t tile, bool more) {
+        const uint64_t db = desc_2 + (tile >> 4);
+#pragma unroll
+        for (int ks = 0; ks < BN / 16; ++ks) umma_f16_ts(acc, src + (ks >> 1) * 32 + (ks & 1) * 8, db + ks * 128, idesc_2, more || ks != 0);
+      };
+      bool ok = wait(F::B_R, 0);
       auto first_stage = [&](int j) -> bool {
         const int buf = j & 1, st1 = j % F::S1, st2 = j % F::S2, left = end - column(j);
         const uint32_t t1 = s1_s + st1 * F::C_TILE, t2 = s2_s + st2 * F::C_TILE;
-        if (!mbar_wait_warp(bar(F::B_2F + st2), (j / F::S2) & 1, abort_flag, p.err, ERR_WAIT_FULL)) return false;
+        if (!wait((F::JOINT ? F::B_1F + st1 : F::B_2F + st2), F::JOINT ? (j / F::S1) & 1 : (j / F::S2) & 1)) return false;
         if (left < BN && KEY_ROWS) ragged_wipe(t2, left, BN, DC);
+        if (F::JOINT && left < BN) ragged_wipe(t1, left, BN, DC);
         tc_fence_after();
-        if (F::DPROD) {
-          if (issuer) {
-            product(tmem + F::DP_COL + buf * BN, r2_s, t2);
-            if (MODE == RB_DQ || MODE == RB_DK) umma_commit(bar(F::B_2E + st2));
-          }
-          __syncwarp();
+        if (F::DPROD && issuer) {
+          product(tmem + F::DP_COL + buf * BN, r2_s, t2);
+          if (!F::JOINT) umma_commit(bar(F::B_2E + st2));
         }
-        if (!mbar_wait_warp(bar(F::B_1F + st1), (j / F::S1) & 1, abort_flag, p.err, ERR_WAIT_FULL)) return false;
-        if (left < BN) ragged_wipe(t1, left, BN, DC);
-        tc_fence_after();
+        if (!F::JOINT) {
+          if (!wait(F::B_1F + st1, (j / F::S1) & 1)) return false;
+          if (left < BN) ragged_wipe(t1, left, BN, DC);
+          tc_fence_after();
+        }
         if (issuer) {
           product(tmem + F::S_COL + buf * BN, r1_s, t1);
           if (MODE == RB_DV) umma_commit(bar(F::B_1E + st1));
@@ -636,22 +715,17 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           if (!ok) break;
         }
         const int buf = j & 1, st1 = j % F::S1, st2 = j % F::S2;
-        ok = mbar_wait_warp(bar(F::B_TR + buf), (j >> 1) & 1, abort_flag, p.err, ERR_WAIT_FULL);
+        ok = wait(F::B_TR + buf, (j >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
         if (issuer) {
-          // 16 columns a step; each half of the 64 columns has its packed values at its own first columns
-          auto second = [&](uint32_t acc, uint32_t src, uint32_t tile) {
-#pragma unroll
-            for (int ks = 0; ks < BN / 16; ++ks)
-              umma_f16_ts(acc, src + buf * BN + (ks >> 1) * 32 + (ks & 1) * 8, make_smem_desc(tile + ks * 2048, F::C_SUB, 1024), idesc_2, (j | ks) != 0);
-          };
           if (MODE == RB_DKV || MODE == RB_DV) {
-            second(tmem + F::ACC, tmem + F::S_COL, s2_s + st2 * F::C_TILE);
-            umma_commit(bar(F::B_2E + st2));
+            second(tmem + F::ACC, tmem + F::S_COL + buf * BN, s2_s + st2 * F::C_TILE, j != 0);
+            if (!F::JOINT) umma_commit(bar(F::B_2E + st2));
           }
           if (F::DPROD) {
-            second(tmem + (MODE == RB_DKV ? F::ACC2 : F::ACC), tmem + F::DP_COL, s1_s + st1 * F::C_TILE);
+            second(tmem + (MODE == RB_DKV ? F::ACC2 : F::ACC), tmem + F::DP_COL + buf * BN, s1_s + st1 * F::C_TILE, j != 0);
+            second(tmem + (MODE == RB_DKV ? F::ACC2 : F::ACC), tmem + F::DP_COL + buf * BN + 16, s1_s + st1 * F::C_TILE, true);
             umma_commit(bar(F::B_1E + st1));
           }
           if (j + 1 == blocks) umma_commit(bar(F::B_ACC));
@@ -664,20 +738,32 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     const int half = (warp - 2) >> 2, quad = warp & 3, r = t.first + quad * 32 + lane;
     const uint32_t lane_at = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float sc = p.scale * FA_LOG2E;
-    const bool fp16 = p.fp16 != 0;
+    constexpr bool fp16 = F16;
     const bool live = KEY_ROWS ? r < t.nk : r < rows;
     const int tok = KEY_ROWS ? 0 : r >> p.pack_log, head = KEY_ROWS ? hk : heads_of(0) + (r & (p.pack - 1));
-    float l2_r = 0.f, dl_r = 0.f;
-    if (!KEY_ROWS && live) {
-      const long long at = static_cast<long long>(t.q0 + tok) * p.Hq + head;
-      l2_r = p.lse[at] * FA_LOG2E;
-      dl_r = p.delta[at];
+    // columns that every row of the tile meets: from plain_lo up to plain_hi
+    int plain_lo, plain_hi;
+    if (KEY_ROWS) {
+      plain_lo = max(0, t.first + 127 - offset) << p.pack_log;
+      plain_hi = p.window > 0 ? static_cast<int>(min(static_cast<long long>(rows), max(0ll, static_cast<long long>(t.first) - offset + p.window) << p.pack_log)) : rows;
+    } else {
+      plain_hi = min(t.nk, (t.first >> p.pack_log) + offset + 1);
+      plain_lo = p.window > 0 ? max(0, ((t.first + 127) >> p.pack_log) + offset - p.window + 1) : 0;
     }
+    float2 own = make_float2(0.f, 0.f);
+    if (!KEY_ROWS && live) own = p.stats[static_cast<long long>(t.q0 + tok) * p.Hq + head];
     bool ok = true;
     for (int j = 0; j < blocks && ok; ++j) {
-      const int buf = j & 1, b0 = column(j), c0 = b0 + half * 32;
+      const int buf = j & 1, b0 = column(j), c0 = b0 + half * 32, st = j % F::NST;
+      float4 col[KEY_ROWS ? 16 : 1];                // statistics of this half's columns, two columns a piece, while the products run
+      if (KEY_ROWS) {
+        ok = mbar_wait_warp(bar(F::B_ST + st), (j / F::NST) & 1, abort_flag, p.err, ERR_WAIT_FULL);
+        if (!ok) break;
+        const float4* sb = reinterpret_cast<const float4*>(stats + st * BN + half * 32);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) col[i] = sb[i];
+      }
       ok = mbar_wait_warp(bar(F::B_SP + buf), (j >> 1) & 1, abort_flag, p.err, ERR_WAIT_TMEM_FULL);
-      if (ok && KEY_ROWS) ok = mbar_wait_warp(bar(F::B_ST + buf), (j >> 1) & 1, abort_flag, p.err, ERR_WAIT_FULL);
       if (!ok) break;
       tc_fence_after();
       const uint32_t s_at = lane_at + F::S_COL + buf * BN + half * 32, d_at = lane_at + F::DP_COL + buf * BN + half * 32;
@@ -685,49 +771,59 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
       tmem_ld_32x32(s_at, x);
       if (F::DPROD) tmem_ld_32x32(d_at, y);
       tmem_wait_ld();
-      const float* sb = stats + buf * 2 * BN + half * 32;
-      // ---- which of the 32 columns this row meets: bits
+      // ---- which of the 32 columns this row meets: bits, where a row of the tile does not meet the whole block
       uint32_t vis = 0xffffffffu;
-      auto below = [](int k) { return k <= 0 ? 0u : (k >= 32 ? 0xffffffffu : (1u << k) - 1u); };
-      if (KEY_ROWS) {
-        // queries (packed) from the one that stands at this key on; with a window up to the last that reaches back to it
-        const int from = max(0, r - offset) << p.pack_log;
-        long long to = rows;
-        if (p.window > 0) to = min(to, max(0ll, static_cast<long long>(r) - offset + p.window) << p.pack_log);
-        vis = live ? below(static_cast<int>(to) - c0) & ~below(from - c0) : 0u;
-      } else {
-        const int last = min(t.nk - 1, tok + offset), from = p.window > 0 ? tok + offset - p.window + 1 : 0;
-        vis = live ? below(last - c0 + 1) & ~below(from - c0) : 0u;
-      }
-      float e[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) e[i] = exp2f(fmaf(__uint_as_float(x[i]), sc, -(KEY_ROWS ? sb[i] : l2_r)));
-      if (vis != 0xffffffffu) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (!((vis >> i) & 1u)) e[i] = 0.f;
-      }
-      if (MODE == RB_DKV || MODE == RB_DV) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = fa_pack2(e[2 * i], e[2 * i + 1], fp16);
-        tmem_st_32x16(s_at, w);
-      }
-      if (F::DPROD) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float d = e[i] * (__uint_as_float(y[i]) - (KEY_ROWS ? sb[BN + i] : dl_r));
-          e[i] = (vis >> i) & 1u ? d : 0.f;         // where no weight is, dP may be anything
+      const bool all = b0 >= plain_lo && b0 + BN <= plain_hi;
+      if (!all) {
+        auto below = [](int k) { return k <= 0 ? 0u : (k >= 32 ? 0xffffffffu : (1u << k) - 1u); };
+        if (KEY_ROWS) {
+          // queries (packed) from the one that stands at this key on; with a window up to the last that reaches back to it
+          const int from = max(0, r - offset) << p.pack_log;
+          long long to = rows;
+          if (p.window > 0) to = min(to, max(0ll, static_cast<long long>(r) - offset + p.window) << p.pack_log);
+          vis = live ? below(static_cast<int>(to) - c0) & ~below(from - c0) : 0u;
+        } else {
+          const int last = min(t.nk - 1, tok + offset), from = p.window > 0 ? tok + offset - p.window + 1 : 0;
+          vis = live ? below(last - c0 + 1) & ~below(from - c0) : 0u;
         }
+      }
+      uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = fa_pack2(e[2 * i], e[2 * i + 1], fp16);
-        tmem_st_32x16(d_at, w);
+      for (int i = 0; i < 16; ++i) {
+        const float4 two = KEY_ROWS ? col[i] : make_float4(own.x, own.x, own.y, own.y);
+        float2 e = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc, make_float2(two.x, two.y));
+        e.x = exp2f(e.x);
+        e.y = exp2f(e.y);
+        if (MODE == RB_DKV || MODE == RB_DV) w[i] = fa_pack2(e.x, e.y, fp16);
+        if (F::DPROD)
+          split2<F16>(mul2(e, add2(make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), make_float2(two.z, two.w))), y[2 * i], y[2 * i + 1]);
+      }
+      if (!all) {                                   // what is not met counts as zero, whatever came out
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t keep = ((vis >> (2 * i)) & 1u ? 0xffffu : 0u) | ((vis >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
+          if (MODE == RB_DKV || MODE == RB_DV) w[i] &= keep;
+          if (F::DPROD) {
+            y[2 * i] &= keep;
+            y[2 * i + 1] &= keep;
+          }
+        }
+      }
+      if (MODE == RB_DKV || MODE == RB_DV) tmem_st_32x16(s_at, w);
+      if (F::DPROD) {
+        uint32_t z[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { z[i] = y[2 * i]; w[i] = y[2 * i + 1]; }
+        tmem_st_32x16(d_at, z);
+        tmem_st_32x16(d_at + 16, w);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(F::B_TR + buf));
+      if (lane == 0) {
+        mbar_arrive(bar(F::B_TR + buf));
+        if (KEY_ROWS) mbar_arrive(bar(F::B_SE + st));
+      }
     }
     if (ok && blocks > 0) {
       ok = mbar_wait_warp(bar(F::B_ACC), 0, abort_flag, p.err, ERR_WAIT_TMEM_FULL);
@@ -793,26 +889,32 @@ static void ragged_bind() {
   if (!bound) { cudaFree(nullptr); bound = true; }
 }
 
-template <int DP>
+template <int DP, bool F16>
 static int ragged_fwd_launch(const CUtensorMap* m, const RaggedParams& p, cudaStream_t stream) {
   using F = RaggedFwd<DP>;
   static_assert(F::SMEM <= 232448, "shared memory budget of one CTA");
   static unsigned long long ready = 0;
-  if (const int rc = ragged_ready(ragged_fwd_kernel<DP>, F::SMEM, &ready)) return rc;
+  if (const int rc = ragged_ready(ragged_fwd_kernel<DP, F16>, F::SMEM, &ready)) return rc;
   const long long tiles = ((p.Tq << p.pack_log) + F::ROWS - 1) / F::ROWS + p.B + 2;
-  ragged_fwd_kernel<DP><<<dim3(static_cast<unsigned>(tiles), p.Hk * p.subs), F::THREADS, F::SMEM, stream>>>(m[0], m[1], m[2], p);
+  ragged_fwd_kernel<DP, F16><<<dim3(static_cast<unsigned>(tiles), p.Hk * p.subs), F::THREADS, F::SMEM, stream>>>(m[0], m[1], m[2], p);
   return static_cast<int>(cudaGetLastError());
 }
-template <int DP, int MODE>
-static int ragged_bwd_launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& s1, const CUtensorMap& s2, const RaggedParams& p,
+template <int DP, int MODE, bool F16>
+static int ragged_bwd_any(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& s1, const CUtensorMap& s2, const RaggedParams& p,
                              cudaStream_t stream) {
   using F = RaggedBwd<DP, MODE>;
   static_assert(F::SMEM <= 232448, "shared memory budget of one CTA");
   static unsigned long long ready = 0;
-  if (const int rc = ragged_ready(ragged_bwd_kernel<DP, MODE>, F::SMEM, &ready)) return rc;
+  if (const int rc = ragged_ready(ragged_bwd_kernel<DP, MODE, F16>, F::SMEM, &ready)) return rc;
   const long long rows = F::KEY_ROWS ? p.Tk : p.Tq << p.pack_log, tiles = (rows + 127) / 128 + p.B + 2;
-  ragged_bwd_kernel<DP, MODE><<<dim3(static_cast<unsigned>(tiles), F::KEY_ROWS ? p.Hk : p.Hk * p.subs), F::THREADS, F::SMEM, stream>>>(r1, r2, s1, s2, p);
+  ragged_bwd_kernel<DP, MODE, F16><<<dim3(static_cast<unsigned>(tiles), F::KEY_ROWS ? p.Hk : p.Hk * p.subs), F::THREADS, F::SMEM, stream>>>(r1, r2, s1, s2, p);
   return static_cast<int>(cudaGetLastError());
+}
+
+template <int DP, int MODE>
+static int ragged_bwd_launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& s1, const CUtensorMap& s2, const RaggedParams& p,
+                             cudaStream_t stream) {
+  return p.fp16 ? ragged_bwd_any<DP, MODE, true>(r1, r2, s1, s2, p, stream) : ragged_bwd_any<DP, MODE, false>(r1, r2, s1, s2, p, stream);
 }
 
 }  // namespace oslo
@@ -830,19 +932,19 @@ extern "C" int oslo_ragged_fwd(const void* q, const void* k, const void* v, void
   if (const int rc = ragged_check(p)) return rc;
   if ((reinterpret_cast<uintptr_t>(o) & 15) || o_sr % 8 || o_sh % 8) return -4;
   ragged_bind();
-  const int bn = D <= 128 ? 128 : 64;
+  const int bn = 64;
   CUtensorMap m[3];
   int rc;
   if ((rc = ragged_map(&m[0], q, D, Hq, Tq, q_sh, q_sr, p.pack, 128 / p.pack, p.fp16))) return rc;
   if ((rc = ragged_map(&m[1], k, D, Hk, Tk, k_sh, k_sr, 1, bn, p.fp16))) return rc;
   if ((rc = ragged_map(&m[2], v, D, Hk, Tk, v_sh, v_sr, 1, bn, p.fp16))) return rc;
-  if (D <= 64) return ragged_fwd_launch<64>(m, p, stream);
-  if (D <= 128) return ragged_fwd_launch<128>(m, p, stream);
-  return ragged_fwd_launch<256>(m, p, stream);
+  if (D <= 64) return p.fp16 ? ragged_fwd_launch<64, true>(m, p, stream) : ragged_fwd_launch<64, false>(m, p, stream);
+  if (D <= 128) return p.fp16 ? ragged_fwd_launch<128, true>(m, p, stream) : ragged_fwd_launch<128, false>(m, p, stream);
+  return p.fp16 ? ragged_fwd_launch<256, true>(m, p, stream) : ragged_fwd_launch<256, false>(m, p, stream);
 }
 
-// delta: workspace [Tq, Hq]
-extern "C" int oslo_ragged_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, float* delta,
+// stats: workspace [Tq, Hq, 2]
+extern "C" int oslo_ragged_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, float* stats,
                                void* dq, void* dk, void* dv, const int* q_off, const int* k_off, int B, int Hq, int Hk, long long Tq,
                                long long Tk, int D, long long q_sr, long long q_sh, long long k_sr, long long k_sh, long long v_sr,
                                long long v_sh, long long o_sr, long long o_sh, long long g_sr, long long g_sh, long long dq_sr,
@@ -851,7 +953,7 @@ extern "C" int oslo_ragged_bwd(const void* q, const void* k, const void* v, cons
   using namespace oslo;
   RaggedParams p{};
   p.q_off = q_off; p.k_off = k_off; p.B = B; p.Hq = Hq; p.Hk = Hk; p.Tq = Tq; p.Tk = Tk; p.D = D; p.window = window; p.scale = scale;
-  p.lse = const_cast<float*>(lse); p.delta = delta; p.err = err_word;
+  p.stats = reinterpret_cast<const float2*>(stats); p.err = err_word;
   if (dtype != OSLO_DT_BF16 && dtype != OSLO_DT_FP16) return -3;
   p.fp16 = dtype == OSLO_DT_FP16;
   if (const int rc = ragged_check(p)) return rc;
@@ -866,8 +968,8 @@ extern "C" int oslo_ragged_bwd(const void* q, const void* k, const void* v, cons
     const int lpr = D <= 64 ? 8 : (D <= 128 ? 16 : 32);
     const long long blocks = (rows + 256 / lpr - 1) / (256 / lpr);
     if (blocks > 0x7fffffffll) return -1;
-#define RAGGED_DELTA(T, L) ragged_delta_kernel<T, L><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T*>(o), static_cast<const T*>(dout), \
-                                                                                                     delta, rows, Hq, D, o_sr, o_sh, g_sr, g_sh)
+#define RAGGED_DELTA(T, L) ragged_delta_kernel<T, L><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T*>(o), static_cast<const T*>(dout), lse, \
+                                                                                                     reinterpret_cast<float2*>(stats), rows, Hq, D, o_sr, o_sh, g_sr, g_sh)
     if (p.fp16) {
       if (lpr == 8) RAGGED_DELTA(__half, 8);
       else if (lpr == 16) RAGGED_DELTA(__half, 16);
