@@ -19,7 +19,8 @@ namespace oslo {
 // ---------------------------------------------------------------------------------------------------------------- append and read
 // Vectors in the order (row, head), keys and values by different blocks (gridDim.y); a group of LPV lanes (8 values each) moves one. Both
 // kernels are bound by memory, as long as a vector's way is found in a few instructions: a block looks its rows' places up once (a search
-// in `offsets`), and a group walks from vector to vector without dividing. U vectors are on their way at a time.
+// in `offsets`), and a group walks from vector to vector without dividing. U vectors are on their way at a time. 8104 rows of 8 heads of 128
+// into 8 bits: 15 us (3.3 TB/s; 39 with a division per vector); 65000 rows from 8 bits: 73 us (5.5 TB/s; 153), from 16 bits 85 us (6.2 TB/s).
 struct PagedMove {
   const void* k; const void* v;             // append: [T, heads, D] by strides (row, head)
   void* ko; void* vo;                       // read: [T, heads, D], contiguous

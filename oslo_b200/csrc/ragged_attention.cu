@@ -204,7 +204,7 @@ __device__ __forceinline__ void ragged_store(uint32_t acc, int from, int to, boo
 // ---------------------------------------------------------------------------------------------------------------- forward
 // MT tiles of 128 rows per CTA. D <= 128: two, with a softmax warpgroup each (thread = row), so that the tensor core works for one tile
 // while the other's exponentials run. S of two blocks of 64 keys per tile: Q K^T of the next block runs under the softmax of this one (with
-// blocks of 128 keys TMEM holds one S a tile; its Q K^T then waited for P V: 350 us instead of 312 for 2 x 4096 tokens, 32/8 heads of
+// blocks of 128 keys TMEM holds one S a tile; its Q K^T then waited for P V: 350 us instead of 304 for 2 x 4096 tokens, 32/8 heads of
 // 128). P overwrites S. Warp 0: TMA; a warp a tile issues its products; then a warpgroup a tile for the softmax. A wait that is over at once
 // still takes 100 to 200 cycles and a commit not much less, so an issuer has two of each a block: K of the next block and V of this one
 // share a stage (with one warp for both tiles and five waits and commits a tile: 449 us).
@@ -527,6 +527,12 @@ enum : int { RB_DKV = 0, RB_DV = 1, RB_DK = 2, RB_DQ = 3 };
 // 128 resident rows (TMEM lane = row), blocks of 64 streamed columns. S and dP of two blocks in TMEM; two warpgroups transform one half
 // of the columns each: P and dS go back, packed, into the half they came from. Head sizes of 256 take dV and dK in two launches: both
 // accumulators fill TMEM alone. r1, s1: what S is made of; r2, s2: what dP (and dV) is made of.
+//
+// 2 x 4096 tokens, 32/8 heads: 1343 us with heads of 128, 1047 with 64, 3318 with 256 (a block of dK and dV takes 2240 cycles with 128, of
+// which its products need 1540: S and dP have 64 columns, which the tensor core takes at three quarters of its rate, since both
+// operands come from shared memory). Per block one wait and one commit fewer (JOINT), the statistics brought by a warp of their own and a
+// uniform test for blocks without a mask: 1278 instead of 1450. Exponentials on the FMA pipe do not pay here (1408 instead of 1363): the
+// transform is bound by its instructions, which is why two values at a time are multiplied and added.
 template <int DP, int MODE> struct RaggedBwd {
   static constexpr bool KEY_ROWS = MODE != RB_DQ, DPROD = MODE != RB_DV;        // DPROD: dP is needed
   static constexpr int BN = 64, DC = DP / 64, THREADS = 64 + 256 + (KEY_ROWS ? 32 : 0), NST = DP == 256 ? 2 : 4;    // NST: blocks of statistics
@@ -874,8 +880,9 @@ template <typename K> static int ragged_ready(K kernel, uint32_t smem, unsigned 
   return 0;
 }
 static int ragged_check(RaggedParams& p) {
-  if (p.B <= 0 || p.Hq <= 0 || p.Hk <= 0 || p.Hq % p.Hk || p.Tq <= 0 || p.Tk <= 0 || p.Tq > 0x7fffffff || p.Tk > 0x7fffffff) return -1;
+  if (p.B <= 0 || p.Hq <= 0 || p.Hk <= 0 || p.Hq % p.Hk || p.Tq <= 0 || p.Tk <= 0 || p.Tq + p.Tk > 0x7fffffff) return -1;      // places of queries among keys are ints
   if (p.D <= 0 || p.D > 256 || p.D % 8) return -2;
+  if (p.window >= p.Tk) p.window = 0;                // it reaches every key
   const int group = p.Hq / p.Hk;
   p.pack = 1;
   p.pack_log = 0;

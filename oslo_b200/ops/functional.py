@@ -407,7 +407,8 @@ def paged_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
     ``k_scale`` and ``v_scale`` ``[pages, kv_heads, page]`` (a vector's largest magnitude over 448). ``page_table`` (int32
     ``[B, columns]``) names a sequence's pages in order; ``lengths`` (int32 ``[B]``) counts its tokens, the new ones among them.
     Sequence ``b``'s new tokens are the rows ``offsets[b]`` to ``offsets[b + 1] - 1``, its last ones (``None``: one row per sequence).
-    A sequence without a length, a position without a page and rows of no sequence are passed over. No gradients."""
+    A sequence without a length, a position without a page and rows of no sequence are passed over. On a GPU: bf16 or fp16 keys and values,
+    heads of a multiple of 8 values (16 in 8-bit pools) up to 256. No gradients."""
     kernels = _kernels(k)
     if kernels is not None:
         return kernels.paged_append(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scale, v_scale)

@@ -202,6 +202,12 @@ def test_ragged_second_derivatives_are_refused():
         torch.autograd.grad(g.float().sum(), leaves[1])
 
 
+@pytest.mark.parametrize("window", [131, 2 ** 31 - 1])
+def test_ragged_windows_wider_than_all_keys(window):
+    # more queries than keys: the first ones stand ahead of every key, and a window reaches far beyond those
+    ragged_case(4, 2, 64, [260, 9], [-200, 62], window=window, seed=77)
+
+
 @pytest.mark.parametrize("bad", [dict(offsets=torch.tensor([0, 5])), dict(offsets=torch.tensor([0, 5]), move=True), dict(scale=-1.0), dict(window=-1), dict(heads=3),
                                  dict(key_offsets=(0, 2, 5)), dict(offsets=torch.tensor([0, 5], dtype=torch.int32))])
 def test_ragged_refusals(bad):
