@@ -729,7 +729,7 @@ extern "C" int oslo_paged_attn(const void* q, long long q_sb, long long q_sh, co
                                int num_sms, cudaStream_t stream) {
   if (B <= 0 || H <= 0 || heads <= 0 || H % heads || D <= 0 || D > 256 || D % 8 || page <= 0 || columns <= 0 || pages <= 0) return -1;
   if (B > 65535 || heads * ((H / heads + 15) / 16) > 65535) return -1;
-  if (static_cast<long long>(columns) * page > 0x7fffffffll) return -1;
+  if (static_cast<long long>(columns) * page > 0x7fff0000ll) return -1;      // a warp looks a batch of keys past the last one
   oslo::PagedAttn p{};
   p.q = q; p.q_sb = q_sb; p.q_sh = q_sh; p.kp = k_pages; p.vp = v_pages; p.ks = k_scale; p.vs = v_scale; p.o = o; p.table = table;
   p.lengths = lengths; p.err = err_word; p.pages = pages; p.scale = scale; p.H = H; p.heads = heads; p.group = H / heads; p.D = D;

@@ -169,34 +169,47 @@ __device__ __forceinline__ void ragged_wipe(uint32_t tile, int from, int rows, i
   fence_proxy_async_smem();
   __syncwarp();
 }
-// lanes 0-31 of the calling warp's TMEM quarter hold a row each: columns [from, to) of its accumulator (zeros where `empty`), times
-// `mult`, into a row of the result (D columns; `live` rows only)
+// Lanes 0-31 of the calling warp's TMEM quarter hold a row each: columns [from, to) of its accumulator (zeros where `empty`), times
+// `mult`, into a row of the result (D columns; `live` rows only). 32 columns of 32 rows pass through `stage`, 2 KB of shared memory that
+// nothing else uses any more, so that four lanes write 64 bytes of a row and eight rows are met at a time (a lane a row met 32, at 5000
+// cycles a tile of 128 columns). Piece c of row r lies at c ^ (r / 2 % 4), which keeps both directions free of bank conflicts.
 __device__ __forceinline__ void ragged_store(uint32_t acc, int from, int to, bool filled, bool empty, float mult, uint16_t* row, int D, bool live,
-                                             bool fp16) {
+                                             bool fp16, uint32_t stage) {
+  if (!filled) {                            // no products, perhaps with copies on their way to where the stage is
+    if (live)
+      for (int c = from; c < to && c < D; c += 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  const uint32_t alive = __ballot_sync(0xffffffffu, live);
 #pragma unroll 1
   for (int c0 = from; c0 < to; c0 += 32) {
     uint32_t r[32];
-    if (filled) {
-      tmem_ld_32x32(acc + c0, r);
-      tmem_wait_ld();
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) r[i] = 0u;
-    }
-    if (!live) continue;
+    tmem_ld_32x32(acc + c0, r);
+    tmem_wait_ld();
     if (empty) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) r[i] = 0u;
     }
+    __syncwarp();                           // the columns before these have been read
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      if (c0 + i >= D) break;
+    for (int c = 0; c < 4; ++c) {
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = fa_pack2(__uint_as_float(r[8 * c + 2 * i]) * mult, __uint_as_float(r[8 * c + 2 * i + 1]) * mult, fp16);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                   "r"(v[3]) : "memory");
+    }
+    __syncwarp();
+    const int c = lane & 3, col = c0 + 8 * c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 8 * i + (lane >> 2);   // the row this lane writes a piece of
+      uint16_t* out = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), at));
       uint4 v;
-      v.x = fa_pack2(__uint_as_float(r[i]) * mult, __uint_as_float(r[i + 1]) * mult, fp16);
-      v.y = fa_pack2(__uint_as_float(r[i + 2]) * mult, __uint_as_float(r[i + 3]) * mult, fp16);
-      v.z = fa_pack2(__uint_as_float(r[i + 4]) * mult, __uint_as_float(r[i + 5]) * mult, fp16);
-      v.w = fa_pack2(__uint_as_float(r[i + 6]) * mult, __uint_as_float(r[i + 7]) * mult, fp16);
-      *reinterpret_cast<uint4*>(row + c0 + i) = v;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + at * 64 + ((c ^ (at >> 1 & 3)) << 4))
+                   : "memory");
+      if ((alive >> at & 1u) && col < D) *reinterpret_cast<uint4*>(out + col) = v;
     }
   }
 }
@@ -473,7 +486,7 @@ ragged_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     const long long at = t.q0 + tok;
     const bool seen = ok && n[i] > 0 && live && last >= first && last >= 0;      // a query that sees no key: zeros
     uint16_t* orow = reinterpret_cast<uint16_t*>(p.out) + at * p.o_sr + head * p.o_sh;
-    ragged_store(o_at, 0, DP, ok && n[i] > 0, !seen, seen ? 1.f / l : 0.f, orow, p.D, live, fp16);
+    ragged_store(o_at, 0, DP, ok && n[i] > 0, !seen, seen ? 1.f / l : 0.f, orow, p.D, live, fp16, q_s + i * F::Q_TILE + quad * 2048);
     if (live && p.lse) p.lse[at * p.Hq + head] = seen ? (m + log2f(l)) * FA_LN2 : 0.f;
   }
 
@@ -837,12 +850,13 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     }
     // ---- each warpgroup stores one half of the accumulator's columns
     const bool filled = ok && blocks > 0;
+    const uint32_t stage = r1_s + (half * 4 + quad) * 2048;           // the products have read the resident rows
     const long long at = KEY_ROWS ? t.k0 + r : t.q0 + tok;
     uint16_t* row = reinterpret_cast<uint16_t*>(p.out) + at * p.o_sr + head * p.o_sh;
-    ragged_store(lane_at + F::ACC, half * DP / 2, (half + 1) * DP / 2, filled, false, MODE == RB_DKV || MODE == RB_DV ? 1.f : p.scale, row, p.D, live, fp16);
+    ragged_store(lane_at + F::ACC, half * DP / 2, (half + 1) * DP / 2, filled, false, MODE == RB_DKV || MODE == RB_DV ? 1.f : p.scale, row, p.D, live, fp16, stage);
     if (MODE == RB_DKV) {
       uint16_t* row2 = reinterpret_cast<uint16_t*>(p.out2) + at * p.o2_sr + head * p.o2_sh;
-      ragged_store(lane_at + F::ACC2, half * DP / 2, (half + 1) * DP / 2, filled, false, p.scale, row2, p.D, live, fp16);
+      ragged_store(lane_at + F::ACC2, half * DP / 2, (half + 1) * DP / 2, filled, false, p.scale, row2, p.D, live, fp16, stage);
     }
   }
 
