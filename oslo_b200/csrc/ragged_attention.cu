@@ -217,7 +217,7 @@ __device__ __forceinline__ void ragged_store(uint32_t acc, int from, int to, boo
 // ---------------------------------------------------------------------------------------------------------------- forward
 // MT tiles of 128 rows per CTA. D <= 128: two, with a softmax warpgroup each (thread = row), so that the tensor core works for one tile
 // while the other's exponentials run. S of two blocks of 64 keys per tile: Q K^T of the next block runs under the softmax of this one (with
-// blocks of 128 keys TMEM holds one S a tile; its Q K^T then waited for P V: 350 us instead of 304 for 2 x 4096 tokens, 32/8 heads of
+// blocks of 128 keys TMEM holds one S a tile; its Q K^T then waited for P V: 350 us instead of 298 for 2 x 4096 tokens, 32/8 heads of
 // 128). P overwrites S. Warp 0: TMA; a warp a tile issues its products; then a warpgroup a tile for the softmax. A wait that is over at once
 // still takes 100 to 200 cycles and a commit not much less, so an issuer has two of each a block: K of the next block and V of this one
 // share a stage (with one warp for both tiles and five waits and commits a tile: 449 us).
@@ -226,7 +226,7 @@ template <int DP> struct RaggedFwd {
   static constexpr int FIRST = 1 + MT, THREADS = 32 * (FIRST + 4 * MT), ROWS = 128 * MT;      // FIRST: the first softmax warp
   static constexpr int DC = DP / 64;
   // of 8 pairs of exponentials, those that the FMA pipe computes: 16 a clock come from the special function unit, half of a block's time.
-  // 0, 1, 2, 3 of 8: 315, 305, 304, 305 us for heads of 128, 285, 277, 275, 276 for 64, 521, 525, 535, 539 for 256 (its products wait for
+  // 0, 1, 2, 3 of 8, measured before the results went through shared memory: 315, 305, 304, 305 us for heads of 128, 285, 277, 275, 276 for 64, 521, 525, 535, 539 for 256 (its products wait for
   // one tile's softmax only; the longer chain of the polynomial shows)
   static constexpr int FMA_EXP = DP <= 128 ? 2 : 0;
   static constexpr uint32_t Q_SUB = 128 * 128, Q_TILE = DC * Q_SUB, KV_SUB = BN * 128, KV_TILE = DC * KV_SUB;
@@ -541,10 +541,10 @@ enum : int { RB_DKV = 0, RB_DV = 1, RB_DK = 2, RB_DQ = 3 };
 // of the columns each: P and dS go back, packed, into the half they came from. Head sizes of 256 take dV and dK in two launches: both
 // accumulators fill TMEM alone. r1, s1: what S is made of; r2, s2: what dP (and dV) is made of.
 //
-// 2 x 4096 tokens, 32/8 heads: 1343 us with heads of 128, 1047 with 64, 3318 with 256 (a block of dK and dV takes 2240 cycles with 128, of
+// 2 x 4096 tokens, 32/8 heads: 1332 us with heads of 128, 1047 with 64, 3318 with 256 (a block of dK and dV takes 2240 cycles with 128, of
 // which its products need 1540: S and dP have 64 columns, which the tensor core takes at three quarters of its rate, since both
 // operands come from shared memory). Per block one wait and one commit fewer (JOINT), the statistics brought by a warp of their own and a
-// uniform test for blocks without a mask: 1278 instead of 1450. Exponentials on the FMA pipe do not pay here (1408 instead of 1363): the
+// uniform test for blocks without a mask: 1278 instead of 1450, before dS became two numbers. Exponentials on the FMA pipe do not pay here (1408 instead of 1363): the
 // transform is bound by its instructions, which is why two values at a time are multiplied and added.
 template <int DP, int MODE> struct RaggedBwd {
   static constexpr bool KEY_ROWS = MODE != RB_DQ, DPROD = MODE != RB_DV;        // DPROD: dP is needed

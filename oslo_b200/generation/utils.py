@@ -155,7 +155,7 @@ class GenerationMixin:
         ``fused_sampling=True`` (not in the reference): with ``do_sample`` and one beam, temperature, top-k, top-p, min-p and the draw run in
         ``ops.sample_tokens``, one kernel a token, with ``torch.rand`` numbers. The distribution is the warpers', but for logits that are
         equal at a border (ranked by index here); the tokens of a seed are others than without it. ``min_p`` keeps tokens of at least
-        that share of the largest probability, one beam only.
+        that share of the largest probability; beams refuse it.
 
         ``output_attentions`` / ``output_hidden_states`` with ``return_dict_in_generate=True`` add ``attentions`` /
         ``hidden_states`` to the result: one entry per generated token, each a tuple over the layers, as the reference's
@@ -248,6 +248,8 @@ class GenerationMixin:
             input_ids, model_kwargs = self._expand_inputs_for_generation(input_ids, num_return_sequences, **model_kwargs)
             fused = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p or 0.0) if fused_sampling else None
             return self.sample(input_ids, procs, stops, warper, fused_settings=fused, **common, **model_kwargs)
+        if min_p:
+            raise ValueError("min_p belongs to sampling with one beam")
         bsz = input_ids.shape[0]
         if num_return_sequences > num_beams:
             raise ValueError("num_return_sequences must be <= num_beams")

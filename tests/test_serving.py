@@ -236,3 +236,9 @@ def test_min_p_without_fused_sampling():
     model = tiny()
     ids = torch.arange(6).view(2, 3)
     assert model.generate(ids, do_sample=True, max_length=12, top_k=0, min_p=1.0).tolist() == model.generate(ids, max_length=12).tolist()
+
+
+def test_min_p_with_beams_is_refused():
+    model = tiny()
+    with pytest.raises(ValueError, match="one beam"):
+        model.generate(torch.tensor([[3, 4]]), num_beams=2, do_sample=True, max_length=6, min_p=0.1)
