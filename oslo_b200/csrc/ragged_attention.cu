@@ -226,8 +226,8 @@ template <int DP> struct RaggedFwd {
   static constexpr int FIRST = 1 + MT, THREADS = 32 * (FIRST + 4 * MT), ROWS = 128 * MT;      // FIRST: the first softmax warp
   static constexpr int DC = DP / 64;
   // of 8 pairs of exponentials, those that the FMA pipe computes: 16 a clock come from the special function unit, half of a block's time.
-  // 0, 1, 2, 3 of 8, measured before the results went through shared memory: 315, 305, 304, 305 us for heads of 128, 285, 277, 275, 276 for 64, 521, 525, 535, 539 for 256 (its products wait for
-  // one tile's softmax only; the longer chain of the polynomial shows)
+  // 0, 1, 2, 3 of 8, measured before the results went through shared memory: 315, 305, 304, 305 us for heads of 128, 285, 277, 275, 276
+  // for 64, 521, 525, 535, 539 for 256 (one tile: its products wait for its softmax, and the polynomial's longer chain shows)
   static constexpr int FMA_EXP = DP <= 128 ? 2 : 0;
   static constexpr uint32_t Q_SUB = 128 * 128, Q_TILE = DC * Q_SUB, KV_SUB = BN * 128, KV_TILE = DC * KV_SUB;
   static constexpr int STAGES = DP == 256 ? 2 : (DP == 128 ? 4 : 6);       // of K of block j + 1 and V of block j
