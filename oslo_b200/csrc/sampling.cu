@@ -722,10 +722,12 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleParam
           const u64 end = sp_all<1>(s, tid < all && ahead <= most ? pair : ~0ull, ~0ull, turn, sp_min);
           tau_key = static_cast<uint32_t>(end >> 32);
           tau_idx = 0xffffffffu - static_cast<uint32_t>(end);
-          // each warp's share of what the list keeps of this block's tokens
+          // each warp's share of what the list keeps of this block's tokens; places ahead of the first token and behind the last one
+          // are the neighbours' tokens, which count there
+          const int a0 = max(j0 * PER, pad), a1 = min(j1 * PER, pad + n);
           for (uint32_t i = lane; i < all; i += 32) {
             const int at = static_cast<int>(0xffffffffu - static_cast<uint32_t>(s.pair[i])) - first;
-            if (at >= j0 * PER && at < j1 * PER && s.pair[i] >= end && s.weight[i] >= w_min) kept += s.weight[i];
+            if (at >= a0 && at < a1 && s.pair[i] >= end && s.weight[i] >= w_min) kept += s.weight[i];
           }
           to = floorf(depth(sp_value(tau_key))) + 1.f;
           from = SP_BINS;                                       // all summed
