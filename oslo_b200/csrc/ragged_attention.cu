@@ -129,18 +129,26 @@ __device__ __forceinline__ float2 fma2v(float2 a, float2 b, float c) {
       "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {      // no number stays no number
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // 2^x of two numbers up to 100 on the FMA pipe, to 2.6e-6 of its value: x = n + f with |f| <= 1/2 (n by adding 1.5 * 2^23), 2^f by a
-// polynomial of degree 4 with the least largest relative error (found by reweighted least squares), n into the exponent
+// polynomial of degree 4 with the least largest relative error (found by reweighted least squares), times 2^n. Below -126.5 it is 0 (n is
+// -127 there, whose exponent bits are those of 0), so what a mask hides weighs nothing; what is no number stays so through the polynomial,
+// whatever 2^n its bits make. 2.6e-6 is less than a hundredth of what rounding the weight to fp16 changes next (2^-11), and changes the sum
+// of weights by no more than that share.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
-  x.x = fmaxf(x.x, -125.f);
-  x.y = fmaxf(x.y, -125.f);
+  x.x = max_nan(x.x, -127.f);
+  x.y = max_nan(x.y, -127.f);
   const float2 t = fma2(x, 1.f, 12582912.f), n = fma2(t, 1.f, -12582912.f), f = fma2v(n, make_float2(-1.f, -1.f), 0.f);
   const float2 g = make_float2(x.x + f.x, x.y + f.y);
   float2 e = fma2(g, 0.009570101698774808f, 0.05591786030272724f);
   e = fma2v(e, g, 0.24024744833108522f);
   e = fma2v(e, g, 0.6931218147397942f);
   e = fma2v(e, g, 0.999999261444132f);
-  return make_float2(__uint_as_float(__float_as_uint(e.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(e.y) + (__float_as_uint(t.y) << 23)));
+  return mul2(e, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
 }
 // a and b as 16-bit values and what those lack, as 16-bit values too: together 16 (bf16) or 22 (fp16) bits of them
 template <bool F16> __device__ __forceinline__ void split2(float2 a, uint32_t& hi, uint32_t& lo) {

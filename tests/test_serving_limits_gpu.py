@@ -44,3 +44,59 @@ def test_sampling_counts_a_token_once_where_blocks_meet(vocab, dtype, others):
                 uniform = torch.full((len(some),), u, device="cuda")
                 got = ops.sample_tokens(x, uniform, top_p=0.9)
                 assert torch.equal(got, ops.reference.sample_tokens(x, uniform, **settings_of(top_p=0.9))), (shift, first, u)
+
+
+# ------------------------------------------------------------------------------------------------------------------ packed attention
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+def test_ragged_a_key_that_is_no_number(dim, dtype, what):
+    """Sequence i has one bad value in key i. With NaN rows ahead of it are as they were, bit by bit, and all others are NaN. With an infinity
+    rows whose score becomes plus infinity, or that see no other key, are NaN, and the others as if that key were not there - to the bound
+    of a result of its own, not to the bit: a row's weights are rounded relative to a reference that may follow those of its neighbours,
+    and an infinite score makes that follow."""
+    count, length = 70, 83
+    at = plain.starts([length] * count)
+    q, k, v = (rnd(count * length, h, dim, seed=i, dtype=dtype) for i, h in enumerate((2, 1, 1)))
+    clean = ops.ragged_attention(q, k, v, ints(*at))
+    bad = k.clone()
+    for i in range(count):
+        bad[at[i] + i, 0, 3] = what
+    got = ops.ragged_attention(q, bad, v, ints(*at))
+    seen = plain.visible(length, length, None, "cuda")
+    u = plain.U[dtype]
+    for i in range(count):
+        a, mid, z = at[i], at[i] + i, at[i + 1]
+        if what != what:
+            assert torch.equal(got[a:mid], clean[a:mid]) and got[mid:z].isnan().all()
+            continue
+        assert q[a:z, :, 3].ne(0).all()
+        up = (q[a:z, :, 3].float() * what > 0) & (torch.arange(length, device="cuda") >= i)[:, None]
+        if i == 0:
+            up[0] = True                                # sees nothing else
+        assert torch.equal(got[a:z].isnan().all(-1), up) and torch.equal(got[a:z].isnan().any(-1), up)
+        keep = [j for j in range(length) if j != i]
+        vv = v[a:z, 0].double()[keep]
+        for h in range(2):
+            p = plain.softmax((q[a:z, h].double() @ k[a:z, 0].double().T * dim ** -0.5)[:, keep], seen[:, keep])
+            w = p @ vv
+            over = (got[a:z, h].double() - w).abs() - ((u + plain.SMALL) * (p @ vv.abs()) + u * w.abs() + 2.0 ** -24)
+            assert over[~up[:, h]].max() <= 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("window", [None, 2])
+def test_ragged_a_query_that_is_no_number(dim, dtype, window):
+    """One bad query in each sequence, at its first places too, where a row meets few keys: its row is NaN and no other."""
+    lens = [1] + [20] * 20 + [70, 130]
+    at = plain.starts(lens)
+    where = [0] + list(range(20)) + [66, 129]
+    q, k, v = (rnd(at[-1], h, dim, seed=i, dtype=dtype) for i, h in enumerate((4, 2, 2)))
+    clean = ops.ragged_attention(q, k, v, ints(*at), window=window)
+    rows = torch.tensor([a + w for a, w in zip(at, where)], device="cuda")
+    q[rows, :, 5] = float("nan")
+    got = ops.ragged_attention(q, k, v, ints(*at), window=window)
+    assert got[rows].isnan().all()
+    others = torch.ones(at[-1], dtype=torch.bool, device="cuda").index_fill_(0, rows, False)
+    assert torch.equal(got[others], clean[others])
