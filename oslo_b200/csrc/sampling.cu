@@ -5,8 +5,9 @@
 //   with w_i >= min_p. All three keep a prefix of the ranks, so what is kept is described by the last one: a (logit, index) pair.
 //   The token is the first in index order whose kept mass, its predecessors' included, exceeds u times the whole kept mass.
 // Masses are whole numbers, w_i * 2^45 rounded (64 bits), so sums do not depend on their order and atomics may add them: the same row
-// always gives the same token, and a sum is compared with its border as 64-bit floating point would compare it, but for 2^-46 of the
-// largest weight per token (a token below that cannot be chosen). exp is evaluated in 64 bits to about 4e-11: table of 2^(j / 16), degree 4.
+// always gives the same token, wherever it starts. exp is evaluated in 64 bits to 4e-11 (table of 2^(j / 16), degree 4), so a weight is off
+// by that share of itself and 2^-46 of the largest (a token below that cannot be chosen), and only a border nearer than that to a sum may
+// fall on its other side.
 //
 // A block, or a cluster of them, holds the row in shared memory; the logits are read once. A small k: the k-th largest of the threads' own
 // largest is a logit that at least k tokens reach, so hardly more than k of them are gathered and the rest happens on that list. Else ranks
@@ -14,7 +15,7 @@
 // top-p by bounds on a bin's mass; one pass sums exact masses, bin by bin inside the bracket; the tokens of the one bin left are ranked
 // against each other (up to 512 of them; more are counted in finer bins first, and equal ones in index order).
 //
-// 512 rows of 50400 bf16 logits: 93 us with top-p 0.9, 31 with top-k 40, 63 without either; one row of 50257: 12 us. Reading them takes 8 us;
+// 512 rows of 50400 bf16 logits: 107 us with top-p 0.9, 29 with top-k 40, 60 without either; one row of 50257: 12 us. Reading them takes 8 us;
 // the rest is shared memory's atomics (the histogram: 6.5 a clock and SM) and the 64-bit exponentials of what may be kept. Two blocks an
 // SM, so that one's waits are the other's work.
 //
@@ -288,8 +289,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleParam
   };
   // f(value, weight, place) for this thread's tokens from `bar` to `roof` (and others, should that be easier), 32 tokens of it at a time.
   // Few of them: a lane takes two at once, one pair after another while any lane of its warp has some; many (over half of some lane's; 12 and
-  // 24 of 32 do as well): four of a piece at once. 512 rows of 50400 bf16 logits, top-p 0.9: 93 us, and 100 where lanes meet after every
-  // piece; with no filter, where all are weighed, 63 and 61.
+  // 24 of 32 do as well): four of a piece at once. 512 rows of 50400 bf16 logits, top-p 0.9: 7 us less than where lanes meet after every
+  // piece; with no filter, where all are weighed, 2 us more.
   constexpr int BATCH = 32 / PER;                               // pieces
   auto weigh = [&](float bar, float roof, auto f) SP_INLINE {
     for (int jb = j0 + lane; jb - lane < j1; jb += 32 * BATCH) {
@@ -613,19 +614,22 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleParam
   if (by_k || by_p) {
     for (int i = tid; i < SP_BINS; i += SP_THREADS) s.count[i] = 0;
     __syncthreads();
-    // top-p's whole: 32-bit exponentials (2^-21), summed as whole numbers. Another last token than in 64 bits, once in a hundred rows or
-    // so, is a token of a hundred-thousandth of the mass more or less, and changes the choice as rarely
-    const float fall = -SP_STEP * 1.44269504f;
+    // top-p's whole in the same pass: its 64-bit exponentials run while the histogram's atomics wait (512 rows of 50400, top-p 0.9: 107 us.
+    // 32-bit ones take 88, but are off by 2^-21, which moves the last token kept in one row of ten; a bound on that error, and the rest of the row
+    // weighed only where the border is nearer, 102 to 106, and 250 instead of 220 at a temperature of 2)
+    const bool weighed = by_p && !by_k;
     for (int j = j0 + lane; j < j1; j += 32) {
-      float v[PER], part = 0.f;
+      float v[PER];
       Piece<T>::get(*reinterpret_cast<const uint4*>(y + j * PER), v);
 #pragma unroll
       for (int c = 0; c < PER; ++c) {
         const float d = depth(v[c]);
-        part += sp_exp2(d * fall);
         if (d < SP_BINS - 1) atomicAdd(&s.count[static_cast<int>(d)], 1u);
       }
-      mass += static_cast<u64>(part * 35184372088832.f);
+      if (weighed) {
+#pragma unroll
+        for (int c = 0; c < PER; ++c) mass += weight(v[c]);
+      }
     }
     sp_sync<C>();
     uint32_t cnt[2] = {0, 0};                                   // of bins 2 tid and 2 tid + 1

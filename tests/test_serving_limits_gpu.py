@@ -46,6 +46,43 @@ def test_sampling_counts_a_token_once_where_blocks_meet(vocab, dtype, others):
                 assert torch.equal(got, ops.reference.sample_tokens(x, uniform, **settings_of(top_p=0.9))), (shift, first, u)
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 50257, torch.float32), (40, 50257, BF16), (300, 5003, torch.float32), (160, 30011, FP16), (6, 131072, torch.float32)])
+@pytest.mark.parametrize("temperature,spread", [(1.0, 2.5), (0.7, 1.0)])
+def test_sampling_at_the_border_of_top_p(rows, vocab, dtype, temperature, spread):
+    """Top-p within half a step of 32 bits (2^-25) of the share at which a token is kept or not. That token has the largest index, so the
+    largest ``uniform`` chooses it if it is kept. What is nearer than 2^-30 is left out: weights are good to 4e-11, some 2^-34."""
+    x = rnd(rows, vocab, seed=rows, scale=spread).to(dtype)
+    last = vocab - 1
+    r = torch.arange(rows, device="cuda")
+    share = torch.tensor([0.3, 0.5, 0.9, 0.97, 0.999], device="cuda", dtype=torch.float64)[r % 5]
+
+    def ahead_of_each(x):
+        order = torch.sort(x.double(), dim=1, descending=True, stable=True).indices
+        w = torch.exp((x.double() - x.double().amax(1, keepdim=True)) / temperature)
+        ranked = torch.gather(w, 1, order)
+        return order, torch.cumsum(ranked, 1) - ranked, w.sum(1, keepdim=True)
+
+    order, ahead, whole = ahead_of_each(x)
+    rank = (ahead < share[:, None] * whole).sum(1).clamp(max=last)          # the first token behind that share
+    token = torch.gather(order, 1, rank[:, None])[:, 0]
+    swapped = x[r, token].clone()
+    x[r, token] = x[:, last].clone()
+    x[:, last] = swapped
+    order, ahead, whole = ahead_of_each(x)
+    at = (order == last).nonzero()[:, 1]
+    border = ahead[r, at] / whole[:, 0]
+    top_p = border.float()
+    told = (top_p.double() - border).abs() > 2.0 ** -30
+    uniform = torch.full((rows,), 1 - 2.0 ** -24, device="cuda")
+    s = settings_of(temperature=temperature, top_p=top_p)
+    want = ops.reference.sample_tokens(x, uniform, **s)
+    assert torch.equal((want == last)[told], (border <= top_p.double())[told])
+    got = ops.sample_tokens(x, uniform, temperature=temperature, top_p=top_p)
+    assert torch.equal(got[told], want[told])
+    s["min_p"] = 1e-7          # the same border
+    assert torch.equal(ops.sample_tokens(x, uniform, **s)[told], ops.reference.sample_tokens(x, uniform, **s)[told])
+
+
 # ------------------------------------------------------------------------------------------------------------------ packed attention
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
