@@ -271,6 +271,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleParam
 
   // what lies outside these is as good as they are, and nothing below overflows
   const double limited = fmin(fmax(temperature, 1e-30), 1e30);
+  if (fabs(static_cast<double>(m)) > 1e6 * limited) {
+    // 32-bit steps at m may be wider than any weight reaches (below, the least logit that has one is a 32-bit number), and m the lowest value
+    // there is, which masks write. Differences from m stand for such logits: exact up to half of m or twice it, and of no weight beyond
+    for (int j = tid; j < pieces * PER; j += SP_THREADS) y[j] = Num<T>::from(value(j) - m);
+    mine_top = Num<T>::to(Num<T>::from(mine_top - m));
+    m = 0.f;
+    __syncthreads();
+  }
   const double inv_t = 1.0 / limited, md = static_cast<double>(m), steps = inv_t * 23.083120654223414;             // 16 / ln 2
   const float per_bin = static_cast<float>(inv_t / SP_STEP), share = static_cast<float>(top_p);
   const float least_v = __double2float_rd(fmax(md - 32.0 * limited, -3.0e38));

@@ -83,6 +83,42 @@ def test_sampling_at_the_border_of_top_p(rows, vocab, dtype, temperature, spread
     assert torch.equal(ops.sample_tokens(x, uniform, **s)[told], ops.reference.sample_tokens(x, uniform, **s)[told])
 
 
+@pytest.mark.parametrize("given", [dict(), dict(top_k=3), dict(top_k=700), dict(top_p=0.6), dict(top_k=700, top_p=0.6), dict(min_p=0.5), dict(temperature=0.0)])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, FP16])
+@pytest.mark.parametrize("vocab", [9, 5003, 50257])
+def test_sampling_rows_of_the_lowest_values(given, dtype, vocab):
+    """Logits at and near the type's lowest value, which masks write, and minus infinity."""
+    low = torch.finfo(dtype).min
+    x = torch.full((8, vocab), low, dtype=dtype, device="cuda")
+    x[1, 1::3] = float("-inf")
+    x[2, 5:] = float("-inf")
+    x[3, ::2] = low * (1 - 2.0 ** -6)
+    x[4] = low * (1 - 0.03125 * torch.rand(vocab, generator=torch.Generator().manual_seed(1))).to(dtype).cuda()
+    x[5, 7] = 0.0
+    x[6, ::5] = -1.0
+    x[7, 2] = low / 2
+    u = torch.tensor([0.5, 0.9, 0.3, 0.7, 0.2, 0.6, 0.99, 0.1], device="cuda")
+    assert torch.equal(ops.sample_tokens(x, u, **given), ops.reference.sample_tokens(x, u, **settings_of(**given)))
+
+
+@pytest.mark.parametrize("given", [dict(), dict(top_k=3), dict(top_k=700), dict(top_p=0.6), dict(top_k=700, top_p=0.6), dict(min_p=0.5)])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, FP16])
+@pytest.mark.parametrize("temperature", [1e-36, 1e-6, 1e-3, 1.0, 1e4])
+def test_sampling_logits_far_larger_than_the_temperature(given, dtype, temperature):
+    """Logits around a value at which 32-bit steps are wider than the temperature, or not so much."""
+    vocab, rows = 5003, 10
+    most = torch.finfo(dtype).max * (1 - 2.0 ** -6)
+    at = torch.tensor([3e38, -3e38, 1e30, -1e20, 1e12, 6e4, -6e4, 1e3, -30.0, 1.0]).clamp(-most, most)
+    x = (at[:, None] * (1 + 2.0 ** -9 * torch.randint(-3, 4, (rows, vocab), generator=torch.Generator().manual_seed(2)))).to(dtype).cuda()
+    x[:, 7::11] = float("-inf")
+    u = torch.tensor([0.5, 0.9, 0.3, 0.7, 0.2, 0.6, 0.99, 0.1, 0.0, 0.45], device="cuda")
+    assert x.isfinite().any(1).all() and not x.isnan().any() and not (x == float("inf")).any()
+    # weights are whole multiples of 2^-45 of the largest: what rounds to none is not chosen, not even by a uniform number of 0
+    weighs = torch.exp((x.double() - x.double().amax(1, keepdim=True)) / temperature) >= 2.0 ** -46
+    want = ops.reference.sample_tokens(x.masked_fill(~weighs, float("-inf")), u, **settings_of(temperature=temperature, **given))
+    assert torch.equal(ops.sample_tokens(x, u, temperature=temperature, **given), want)
+
+
 # ------------------------------------------------------------------------------------------------------------------ packed attention
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
