@@ -445,6 +445,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attn_kernel(const PagedAt
     for (int j = 0; j < 2; ++j) { m[nb][j] = -CUDART_INF_F; l[nb][j] = 0.f; }
   }
   float vref = 0.f, vinv = 0.f;                                   // Q8: the value scales' reference (0: none yet)
+  uint32_t met = 0;                                               // whether this warp has met a key
   int slot = 0;
   for (int tb = t0 + warp * KPS; tb < t1; tb += PA_WARPS * KPS) {
     fetch();                                                      // into the slot of the batch before this one
@@ -482,6 +483,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attn_kernel(const PagedAt
     // ---- scores in log2 units; keys behind the last one, or without a page, have none. This lane's keys: g and g + 8
     uint32_t there;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(there) : "r"(at + S::STAGE - 16) : "memory");
+    met |= there;
     const bool in[2] = {((there >> g) & 1u) != 0, ((there >> (g + 8)) & 1u) != 0};
     float kscale[2] = {1.f, 1.f}, vscale[2] = {1.f, 1.f};
     if constexpr (Q8) {
@@ -602,7 +604,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attn_kernel(const PagedAt
     if (g == 0) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        stat[warp][nb * 8 + 2 * t4 + j][0] = m[nb][j];
+        // no finite score among keys that are there is not the same as no key: it ends in 0 / 0
+        stat[warp][nb * 8 + 2 * t4 + j][0] = met && m[nb][j] == -CUDART_INF_F ? -CUDART_MAX_NORMAL_F : m[nb][j];
         stat[warp][nb * 8 + 2 * t4 + j][1] = l[nb][j];
       }
     }
@@ -639,12 +642,12 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attn_kernel(const PagedAt
   for (int i = split * PA_WARPS * 32 + threadIdx.x; i < nh * DP; i += splits * PA_WARPS * 32) {
     const int row = i / DP, d = i % DP;
     if (d >= p.D) continue;
-    float val, sum;
+    float val, sum, mm = -CUDART_INF_F;
     if (splits == 1) {
+      mm = fin[row][0];
       sum = fin[row][1];
       val = mine[i];
     } else {
-      float mm = -CUDART_INF_F;
       for (int r = 0; r < splits; ++r) mm = fmaxf(mm, peer(fin_s + row * 8, r));
       const float base = mm == -CUDART_INF_F ? 0.f : mm;
       sum = 0.f;
@@ -655,7 +658,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attn_kernel(const PagedAt
         val += f * peer(mine_s + i * 4, r);
       }
     }
-    out[row * p.D + d] = Num<T>::from(sum == 0.f ? 0.f : val / sum);
+    out[row * p.D + d] = Num<T>::from(mm == -CUDART_INF_F ? 0.f : val / sum);      // no key: zeros
   }
   if (splits > 1) cluster_sync_all();                             // nobody leaves while another reads its shared memory
 }

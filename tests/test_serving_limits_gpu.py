@@ -173,3 +173,44 @@ def test_ragged_a_query_that_is_no_number(dim, dtype, window):
     assert got[rows].isnan().all()
     others = torch.ones(at[-1], dtype=torch.bool, device="cuda").index_fill_(0, rows, False)
     assert torch.equal(got[others], clean[others])
+
+
+# ------------------------------------------------------------------------------------------------------------------ pages
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_paged_attention_scores_that_are_infinite_or_no_number(rows, dtype, dim):
+    """Bad keys at each place of a batch. All scores minus infinity, one plus infinity or one no number: NaN. Minus infinity beside finite
+    scores: as without that key. Nothing to see: zeros."""
+    length, page = 150, 16
+    columns = -(-length // page)
+    table = torch.arange(rows * columns, dtype=torch.int32, device="cuda").view(rows, columns)
+    q = rnd(rows, 4, dim, seed=1, dtype=dtype)
+    q[:, :, 3] = 1.0
+    kp, vp = (rnd(rows * columns, 2, page, dim, seed=i, dtype=dtype) for i in (2, 3))
+    lens = torch.full((rows,), length, dtype=torch.int32, device="cuda")
+    clean = ops.paged_attention(q, kp, vp, table, lens)
+    for place in (0, 5, 15, 16, 63, 64, 149):
+        for what in (float("nan"), float("inf"), float("-inf")):
+            bad = kp.clone()
+            bad[table[:, place // page].long(), :, place % page, 3] = what
+            got = ops.paged_attention(q, bad, vp, table, lens)
+            if what != float("-inf"):
+                assert got.isnan().all(), (place, what)
+                continue
+            b = rows - 1
+            k, v = plain.held(kp, None, table, b, length), plain.held(vp, None, table, b, length)
+            keep = [j for j in range(length) if j != place]
+            u = plain.U[dtype]
+            for h in range(4):
+                p = torch.softmax(k[keep, h // 2] @ q[b, h].double() * dim ** -0.5, 0)
+                w, e = p @ v[keep, h // 2], p @ v[keep, h // 2].abs()
+                assert ((got[b, h].double() - w).abs() <= (u + plain.SMALL) * e + u * w.abs() + 2.0 ** -24).all()
+    kp[..., 3] = float("-inf")
+    for n in (1, 17, 150):
+        for window in (None, 3):
+            lens.fill_(n)
+            lens[0] = 0 if rows > 1 else n
+            got = ops.paged_attention(q, kp, vp, table, lens, window=window)
+            assert got[rows > 1:].isnan().all() and (rows == 1 or not got[0].any())
+    assert clean.isfinite().all()
