@@ -71,12 +71,12 @@ std::tuple<Tensor, Tensor, Tensor> ragged_bwd(const Tensor& dout_, const Tensor&
   TORCH_CHECK(o.sizes() == q.sizes() && o.is_contiguous() && dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() &&
                   o.scalar_type() == q.scalar_type() && dout.device() == q.device() && lse.numel() == q.size(0) * q.size(1),
               "ragged_attention: the output and its gradient must be like q");
-  // gradients of slices of one projection's rows are slices of one tensor too, so that nobody has to join them
+  // gradients of slices of one projection's rows are slices of one tensor too, so that nobody has to join them. The given strides alone
+  // decide, not addresses: a trace, which has none, must be told the same layout
   const int64_t D = q.size(2), Wq = q.size(1) * D, Wk = k.size(1) * D, W = Wq + 2 * Wk;
   Tensor dq, dk, dv;
-  const auto* at0 = static_cast<const char*>(q.data_ptr());
-  if (q.size(0) == k.size(0) && q.stride(1) == D && k.stride(1) == D && v.stride(1) == D && q.stride(0) == W && k.stride(0) == W && v.stride(0) == W &&
-      static_cast<const char*>(k.data_ptr()) == at0 + Wq * q.element_size() && static_cast<const char*>(v.data_ptr()) == at0 + (Wq + Wk) * q.element_size()) {
+  auto sliced = [&](const Tensor& t) { return t.stride(0) == W && t.stride(1) == D && t.stride(2) == 1; };
+  if (q.size(0) == k.size(0) && sliced(q_) && sliced(k_) && sliced(v_)) {
     Tensor all = at::empty({q.size(0), W}, q.options());
     dq = all.slice(1, 0, Wq).view(q.sizes());
     dk = all.slice(1, Wq, Wq + Wk).view(k.sizes());

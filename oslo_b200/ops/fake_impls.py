@@ -352,6 +352,10 @@ def register() -> None:
 
     @reg("oslo_b200::ragged_bwd")
     def _(dout, q, k, v, o, lse, offsets, key_offsets, scale, window):
+        d = q.size(2)
+        sizes = [t.size(1) * d for t in (q, k, v)]
+        if q.size(0) == k.size(0) and all(t.stride() == (sum(sizes), d, 1) for t in (q, k, v)):      # slices of one projection
+            return tuple(t.view(q.size(0), -1, d) for t in q.new_empty((q.size(0), sum(sizes))).split(sizes, dim=1))
         return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
     @reg("oslo_b200::paged_append")

@@ -175,6 +175,49 @@ def test_ragged_a_query_that_is_no_number(dim, dtype, window):
     assert torch.equal(got[others], clean[others])
 
 
+def test_ragged_gradients_have_the_strides_that_a_trace_is_told():
+    """Layouts of operands, neighbours in memory or only alike: what the kernel returns is laid out as its shape implementation says."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    heads, kv, dim, rows, at = 4, 2, 64, 30, ints(0, 13, 30)
+    wide = (heads + 2 * kv) * dim
+    x = rnd(rows, wide, dtype=BF16)
+    q, k, v = (t.view(rows, -1, dim) for t in x.split([heads * dim, kv * dim, kv * dim], 1))
+    other = torch.empty(rows, wide, dtype=BF16, device="cuda")[:, 64:64 + kv * dim].view(rows, kv, dim).copy_(k)       # alike, elsewhere
+    odd = torch.empty(rows * wide + 1, dtype=BF16, device="cuda")[1:].view(rows, wide)[:, :kv * dim].view(rows, kv, dim).copy_(k)     # between 16-byte boundaries
+    cases = [(q, k, v), (q.contiguous(), k, v), (q, k.contiguous(), v), (q, other, v), (q, odd, v), (q, v, k), (q.transpose(0, 1).contiguous().transpose(0, 1), k, v)]
+    grads = []
+    for a, b, c in cases:
+        o, lse = torch.ops.oslo_b200.ragged_fwd(a, b, c, at, at, 0.125, 0, True)
+        args = (torch.ones_like(o), a, b, c, o, lse, at, at)
+        real = torch.ops.oslo_b200.ragged_bwd(*args, 0.125, 0)
+        with FakeTensorMode() as mode:
+            told = torch.ops.oslo_b200.ragged_bwd(*(mode.from_tensor(t) for t in args), 0.125, 0)
+        for r, t in zip(real, told):
+            assert r.shape == t.shape and r.stride() == t.stride()
+        grads.append(real)
+    for i in (1, 2, 3, 4, 6):           # the same operands in other places
+        for r, t in zip(grads[i], grads[0]):
+            assert torch.equal(r, t)
+
+
+def test_ragged_traced_training_step_of_a_joint_projection():
+    """Forward and backward as one traced graph, which is told shapes and strides only, against the same step untraced."""
+    heads, kv, dim, rows, at = 4, 2, 64, 48, ints(0, 13, 48)
+    x, w, do = rnd(rows, 96, seed=1, dtype=BF16), rnd(96, (heads + 2 * kv) * dim, seed=2, dtype=BF16, scale=0.1), rnd(rows, heads * dim, seed=3, dtype=BF16)
+
+    def step(x, w, do):
+        q, k, v = (t.view(rows, -1, dim) for t in (x @ w).split([heads * dim, kv * dim, kv * dim], 1))
+        o = ops.ragged_attention(q, k, v, at).flatten(1)
+        return torch.autograd.grad(o, w, do)[0]
+
+    from torch.fx.experimental.proxy_tensor import make_fx
+    leaf = w.clone().requires_grad_()
+    want = step(x, leaf, do)
+    traced = make_fx(step, tracing_mode="fake", _allow_non_fake_inputs=True)(x, leaf, do)
+    assert any("ragged_bwd" in str(n.target) for n in traced.graph.nodes)
+    assert torch.equal(traced(x, leaf, do), want)
+
+
 # ------------------------------------------------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("rows", [1, 300])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
