@@ -385,12 +385,13 @@ def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
                      scale: Optional[float] = None) -> Tensor:
     """Causal attention of packed sequences with grouped heads: ``q`` ``[T, heads, D]``, ``k`` and ``v`` ``[T_k, kv_heads, D]``.
 
-    Sequence ``b`` has the rows ``offsets[b]`` to ``offsets[b + 1] - 1`` (int32 ``[B + 1]`` on the device, not decreasing; the host never
-    reads them) of ``q``, and those of ``key_offsets`` (default: the same) of ``k`` and ``v``; its last query stands at its last key, so
+    Sequence ``b`` has the rows ``offsets[b]`` to ``offsets[b + 1] - 1`` (int32 ``[B + 1]`` on the device, not decreasing; the kernels
+    alone read them) of ``q``, and those of ``key_offsets`` (default: the same) of ``k`` and ``v``; its last query stands at its last key, so
     cached keys may lie ahead of a prompt that goes on. ``window``: a query sees that many keys, its own place among them. Rows of no
     sequence, and queries that see no key, give zeros. 16-bit CUDA tensors with ``D`` a multiple of 8 up to 256 take the tcgen05
-    kernels, forward and backward; sequences do not touch each other's numbers, whatever those are (a number that is none spoils rows of its own
-    sequence only)."""
+    kernels, forward and backward; other types and sizes are computed sequence by sequence in 32-bit PyTorch operations, on a GPU too, and
+    the host then reads the offsets (which a stream capture refuses). Sequences do not touch each other's numbers, whatever those are (a
+    number that is none spoils rows of its own sequence only)."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.size(-1))
     kernels = _kernels(q)

@@ -711,7 +711,7 @@ def _sequence_of(offsets: Tensor, rows: int) -> Tuple[Tensor, Tensor]:
 
 def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offsets: Optional[Tensor], window: Optional[int],
                      scale: float) -> Tensor:
-    """See ``functional.ragged_attention``; scores of all rows with all keys."""
+    """See ``functional.ragged_attention``; sequence by sequence, so that none meets another's numbers (the host reads the offsets)."""
     if q.dim() != 3 or k.shape != v.shape or k.dim() != 3 or k.size(2) != q.size(2) or k.size(1) == 0 or q.size(1) % k.size(1):
         raise ValueError("ragged_attention: q must be [T, heads, D], k and v [T_k, kv_heads, D] with kv_heads a divisor of heads")
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -721,19 +721,21 @@ def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
         raise ValueError("ragged_attention: offsets are int32 [sequences + 1]")
     if not scale > 0 or (window is not None and window < 0):
         raise ValueError("ragged_attention: the scale must be positive and the window not negative")
-    qs, qi = _sequence_of(offsets, q.size(0))
-    ks, ki = _sequence_of(key_offsets, k.size(0))
-    lens, klens = (o[1:].to(torch.long) - o[:-1].to(torch.long) for o in (offsets, key_offsets))
-    at = qi + (klens - lens)[qs.clamp(min=0)]
-    seen = (qs[:, None] == ks[None]) & (qs >= 0)[:, None] & (ki[None] <= at[:, None])
-    if window:
-        seen &= ki[None] > (at - window)[:, None]
-    group = q.size(1) // k.size(1)
-    kf, vf = (t.float().repeat_interleave(group, dim=1).transpose(0, 1) for t in (k, v))
-    s = torch.matmul(q.float().transpose(0, 1), kf.transpose(1, 2)) * scale
-    p = torch.softmax(s.masked_fill(~seen, float("-inf")), dim=-1)
-    p = torch.where(seen & seen.any(-1, keepdim=True), p, torch.zeros((), dtype=p.dtype, device=p.device))
-    return torch.matmul(p, vf).transpose(0, 1).to(q.dtype)
+    kv = k.size(1)
+
+    def attend(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+        n, m = q.size(0), k.size(0)
+        ahead = torch.arange(m, device=q.device) - (torch.arange(n, device=q.device)[:, None] + m - n)       # of a query's own place
+        seen = (ahead <= 0) & (ahead > -window) if window else ahead <= 0
+        qf, kf, vf = q.float().transpose(0, 1).unflatten(0, (kv, -1)), k.float().permute(1, 2, 0)[:, None], v.float().transpose(0, 1)[:, None]
+        p = torch.softmax((torch.matmul(qf, kf) * scale).masked_fill(~seen, float("-inf")), dim=-1)
+        p = torch.where(seen & seen.any(-1, keepdim=True), p, torch.zeros((), dtype=p.dtype, device=p.device))
+        return torch.matmul(p, vf).flatten(0, 1).transpose(0, 1).to(q.dtype)
+
+    at, key_at = ([min(max(o, 0), t.size(0)) for o in starts.tolist()] for starts, t in ((offsets, q), (key_offsets, k)))
+    # rows ahead of the first sequence and behind the last one: sequences without keys
+    parts = [(0, at[0], 0, 0), *zip(at, at[1:], key_at, key_at[1:]), (at[-1], q.size(0), 0, 0)]
+    return torch.cat([attend(q[a:b], k[c:max(c, d)], v[c:max(c, d)]) for a, b, c, d in parts])
 
 
 def quantise(x: Tensor) -> Tuple[Tensor, Tensor]:

@@ -5,6 +5,14 @@ import torch
 from oslo_b200 import ops
 
 
+def rnd(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed + sum(shape))).to(dtype)
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
 @pytest.mark.parametrize("joint", [True, False])
 def test_ragged_gradients_of_a_trace_have_their_strides(joint):
     """Gradients of slices of one projection are slices of one tensor, also where only shapes are traced; others are contiguous."""
@@ -23,3 +31,31 @@ def test_ragged_gradients_of_a_trace_have_their_strides(joint):
         for g, t in zip(got, (q, k, v)):
             assert g.shape == t.shape and g.dtype == t.dtype
             assert g.stride() == (t.stride() if joint else (t.size(1) * dim, dim, 1))
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_ragged_statement_keeps_sequences_apart(what, dtype):
+    """What is no number in one sequence, or in rows of none, leaves the others as they are - forward and backward."""
+    at = [2, 9, 20, 33]
+    q, k, v, do = (rnd(40, h, 8, seed=i, dtype=dtype) for i, h in enumerate((4, 2, 2, 4)))
+    clean = [t.clone().requires_grad_() for t in (q, k, v)]
+    o1 = ops.ragged_attention(*clean, ints(*at))
+    g1 = torch.autograd.grad(o1, clean, do)
+    for t in (q, k, v, do):
+        t[:2] = t[9:20] = t[33:] = what
+    bad = [t.clone().requires_grad_() for t in (q, k, v)]
+    o2 = ops.ragged_attention(*bad, ints(*at))
+    g2 = torch.autograd.grad(o2, bad, do)
+    for a, b in zip((o1, *g1), (o2, *g2)):
+        assert torch.equal(a[2:9], b[2:9]) and torch.equal(a[20:33], b[20:33])
+        assert not b[:2].any() and not b[33:].any()
+    assert o2[9:20].isnan().all()
+
+
+def test_ragged_statement_without_rows_or_keys():
+    for rows, keys, starts, key_starts in ((0, 5, (0, 0), (0, 5)), (5, 0, (0, 5), (0, 0)), (5, 4, (0, 0, 0), (0, 2, 4)), (3, 4, (0, 1, 3), (0, 4, 4))):
+        leaves = [rnd(rows, 4, 8, seed=1).requires_grad_(), rnd(keys, 2, 8, seed=2).requires_grad_(), rnd(keys, 2, 8, seed=3).requires_grad_()]
+        o = ops.ragged_attention(*leaves, ints(*starts), ints(*key_starts))
+        assert o.shape == leaves[0].shape and o.isfinite().all() and not o[1:].any()
+        assert all(g.isfinite().all() for g in torch.autograd.grad(o.sum(), leaves))

@@ -218,6 +218,19 @@ def test_ragged_traced_training_step_of_a_joint_projection():
     assert torch.equal(traced(x, leaf, do), want)
 
 
+def test_ragged_in_32_bits_on_the_gpu():
+    """Computed sequence by sequence in PyTorch: as on the CPU, to 128 terms of 2^-24 twice over, forward and backward."""
+    at = [0, 5, 5, 90, 131]
+    made = [rnd(140, h, 24, seed=i) for i, h in enumerate((4, 2, 2, 4))]
+    both = []
+    for dev in ("cuda", "cpu"):
+        leaves = [t.to(dev, copy=True).requires_grad_() for t in made[:3]]
+        o = ops.ragged_attention(*leaves, torch.tensor(at, dtype=torch.int32, device=dev), window=40)
+        both.append([t.cpu() for t in (o.detach(), *torch.autograd.grad(o, leaves, made[3].to(dev)))])
+    for a, b in zip(*both):
+        assert (a - b).abs().max() <= plain.SMALL * max(1.0, b.abs().max().item()) * 8          # sums of up to 8 such terms' size
+
+
 # ------------------------------------------------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("rows", [1, 300])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
