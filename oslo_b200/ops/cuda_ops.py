@@ -1152,6 +1152,9 @@ def _op(name: str):
 
 
 def ragged_ok(q: Tensor, k: Tensor, v: Tensor) -> bool:
+    """Whether the kernels take it. Function transforms and forward-mode derivatives cannot look into them and take the statement."""
+    if torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0:
+        return False
     return q.dtype in _16BIT and k.dtype == q.dtype and v.dtype == q.dtype and q.dim() == 3 and q.size(2) % 8 == 0 and q.size(2) <= 256
 
 

@@ -389,9 +389,9 @@ def ragged_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
     alone read them) of ``q``, and those of ``key_offsets`` (default: the same) of ``k`` and ``v``; its last query stands at its last key, so
     cached keys may lie ahead of a prompt that goes on. ``window``: a query sees that many keys, its own place among them. Rows of no
     sequence, and queries that see no key, give zeros. 16-bit CUDA tensors with ``D`` a multiple of 8 up to 256 take the tcgen05
-    kernels, forward and backward; other types and sizes are computed sequence by sequence in 32-bit PyTorch operations, on a GPU too, and
-    the host then reads the offsets (which a stream capture refuses). Sequences do not touch each other's numbers, whatever those are (a
-    number that is none spoils rows of its own sequence only)."""
+    kernels, forward and backward; other types and sizes, function transforms and forward-mode derivatives are computed sequence by sequence
+    in 32-bit PyTorch operations, on a GPU too, and the host then reads the offsets (which a stream capture refuses). Sequences do not touch
+    each other's numbers, whatever those are (a number that is none spoils rows of its own sequence only)."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.size(-1))
     kernels = _kernels(q)

@@ -175,6 +175,28 @@ def test_ragged_a_query_that_is_no_number(dim, dtype, window):
     assert torch.equal(got[others], clean[others])
 
 
+def test_ragged_under_function_transforms():
+    """Forward-mode derivatives and ``torch.func.grad`` against those of the double-precision formula; never a silent zero. Sums are 32-bit, the
+    result is rounded to fp16: half a step is 2^-11 of a value."""
+    at = [0, 13, 40]
+    q, k, v, t = (rnd(40, h, 16, seed=i, dtype=FP16) for i, h in enumerate((4, 2, 2, 4)))
+
+    def formula(x, kk, vv):
+        return torch.cat([torch.cat([plain.softmax(x[a:z, h] @ kk[a:z, h // 2].T / 4, plain.visible(z - a, z - a, None, "cuda")) @ vv[a:z, h // 2]
+                                     for h in range(4)], 1).unflatten(1, (4, 16)) for a, z in zip(at, at[1:])])
+
+    _, want = torch.func.jvp(lambda x: formula(x, k.double(), v.double()), (q.double(),), (t.double(),))
+    _, got = torch.func.jvp(lambda x: ops.ragged_attention(x, k, v, ints(*at)), (q,), (t,))
+    assert want.abs().max() > 0.1 and (got.double() - want).abs().max() < 2.0 ** -10 * max(1.0, want.abs().max().item())
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, t)
+        tangent = torch.autograd.forward_ad.unpack_dual(ops.ragged_attention(dual, k, v, ints(*at))).tangent
+    assert torch.equal(tangent, got)
+    want = torch.func.grad(lambda x: (formula(x, k.double(), v.double()) * t.double()).sum())(q.double())
+    got = torch.func.grad(lambda x: (ops.ragged_attention(x, k, v, ints(*at)).float() * t.float()).sum())(q)
+    assert (got.double() - want).abs().max() < 2.0 ** -10 * max(1.0, want.abs().max().item())
+
+
 def test_ragged_gradients_have_the_strides_that_a_trace_is_told():
     """Layouts of operands, neighbours in memory or only alike: what the kernel returns is laid out as its shape implementation says."""
     from torch._subclasses.fake_tensor import FakeTensorMode
