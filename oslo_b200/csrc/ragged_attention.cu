@@ -180,14 +180,17 @@ __device__ __forceinline__ void ragged_wipe(uint32_t tile, int from, int rows, i
 // Lanes 0-31 of the calling warp's TMEM quarter hold a row each: columns [from, to) of its accumulator (zeros where `empty`), times
 // `mult`, into a row of the result (D columns; `live` rows only). 32 columns of 32 rows pass through `stage`, 2 KB of shared memory that
 // nothing else uses any more, so that four lanes write 64 bytes of a row and eight rows are met at a time (a lane a row met 32, at 5000
-// cycles a tile of 128 columns). Piece c of row r lies at c ^ (r / 2 % 4), which keeps both directions free of bank conflicts.
-__device__ __forceinline__ void ragged_store(uint32_t acc, int from, int to, bool filled, bool empty, float mult, uint16_t* row, int D, bool live,
+// cycles a tile of 128 columns). Piece c of row r lies at c ^ (r / 2 % 4), which keeps both directions free of bank conflicts. CHECK: whether
+// a value of this lane's row is infinite or no number.
+template <bool CHECK = false>
+__device__ __forceinline__ bool ragged_store(uint32_t acc, int from, int to, bool filled, bool empty, float mult, uint16_t* row, int D, bool live,
                                              bool fp16, uint32_t stage) {
   if (!filled) {                            // no products, perhaps with copies on their way to where the stage is
     if (live)
       for (int c = from; c < to && c < D; c += 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
-    return;
+    return false;
   }
+  bool odd = false;
   const int lane = threadIdx.x & 31;
   const uint32_t alive = __ballot_sync(0xffffffffu, live);
 #pragma unroll 1
@@ -198,6 +201,10 @@ __device__ __forceinline__ void ragged_store(uint32_t acc, int from, int to, boo
     if (empty) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) r[i] = 0u;
+    }
+    if (CHECK) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) odd |= (r[i] & 0x7f800000u) == 0x7f800000u;
     }
     __syncwarp();                           // the columns before these have been read
 #pragma unroll
@@ -220,6 +227,7 @@ __device__ __forceinline__ void ragged_store(uint32_t acc, int from, int to, boo
       if ((alive >> at & 1u) && col < D) *reinterpret_cast<uint4*>(out + col) = v;
     }
   }
+  return odd;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- forward
@@ -572,6 +580,11 @@ template <int DP, int MODE> struct RaggedBwd {
   static constexpr uint32_t SMEM = TILES + STATS + BARS * 8 + 64 + 1024;
 };
 
+// fp16: dS may be beyond the type (65504) where dQ and dK are not. A tile whose accumulator has rows that are infinite or no number runs a
+// second time, with dS times 2^-26 (|dP| and |delta| are at most 256 * 65504^2 < 2^40), and writes those rows only. A weight is then off by up
+// to 2, against a largest one of more than 65504. Loss-scaled training gets there; others pay a look at each row's results.
+__device__ __forceinline__ void mbar_inval(uint32_t bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+
 template <int DP, int MODE, bool F16>
 __global__ void __launch_bounds__(RaggedBwd<DP, MODE>::THREADS, 1)
 ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant__ CUtensorMap tr2, const __grid_constant__ CUtensorMap ts1,
@@ -596,10 +609,13 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     const RaggedTile t = ragged_find(p, KEY_ROWS, 128, blockIdx.x);
     if (lane == 0) *found = t;
   }
-  if (threadIdx.x == 32) {
+  auto init_barriers = [&]() {
     for (int i = 0; i < F::BARS; ++i) mbar_init(bar(i), (i >= F::B_TR && i < F::B_TR + 2) || (i >= F::B_SE && i < F::B_SE + F::NST) ? 8 : 1);
-    *abort_flag = 0;
     fence_barrier_init();
+  };
+  if (threadIdx.x == 32) {
+    *abort_flag = 0;
+    init_barriers();
   }
   __syncthreads();
   const RaggedTile t = *found;
@@ -631,6 +647,11 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   auto column = [&](int j) { return c_lo + (KEY_ROWS ? j % per : j) * BN; };
   auto heads_of = [&](int j) { return hk * group + (KEY_ROWS ? j / per : sub0) * p.pack; };
 
+  constexpr bool AGAIN = F16 && F::DPROD;                           // the tile may run a second time
+  float lift = 1.f;                                                 // what dS is multiplied by
+  bool odd = false;                                                 // a row whose result was no number the first time
+#pragma unroll 1
+  for (int turn = 0;; ++turn) {
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && blocks > 0) {
@@ -684,7 +705,7 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
       if (j + 1 < blocks) fetch(j + 1, next);
       const int st = j % F::NST;
       if (!mbar_wait_warp(bar(F::B_SE + st), ((j / F::NST) & 1) ^ 1, abort_flag, p.err, ERR_WAIT_EMPTY)) break;
-      *reinterpret_cast<float4*>(stats + st * BN + lane * 2) = make_float4(now[0].x, now[1].x, now[0].y, now[1].y);
+      *reinterpret_cast<float4*>(stats + st * BN + lane * 2) = make_float4(now[0].x, now[1].x, AGAIN ? now[0].y * lift : now[0].y, AGAIN ? now[1].y * lift : now[1].y);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(F::B_ST + st));
       now[0] = next[0];
@@ -779,6 +800,7 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     }
     float2 own = make_float2(0.f, 0.f);
     if (!KEY_ROWS && live) own = p.stats[static_cast<long long>(t.q0 + tok) * p.Hq + head];
+    if (AGAIN) own.y *= lift;
     bool ok = true;
     for (int j = 0; j < blocks && ok; ++j) {
       const int buf = j & 1, b0 = column(j), c0 = b0 + half * 32, st = j % F::NST;
@@ -822,8 +844,10 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
         e.x = exp2f(e.x);
         e.y = exp2f(e.y);
         if (MODE == RB_DKV || MODE == RB_DV) w[i] = fa_pack2(e.x, e.y, fp16);
-        if (F::DPROD)
-          split2<F16>(mul2(e, add2(make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), make_float2(two.z, two.w))), y[2 * i], y[2 * i + 1]);
+        if (F::DPROD) {
+          const float2 dp = make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), delta = make_float2(two.z, two.w);
+          split2<F16>(mul2(e, AGAIN ? fma2(dp, lift, delta) : add2(dp, delta)), y[2 * i], y[2 * i + 1]);
+        }
       }
       if (!all) {                                   // what is not met counts as zero, whatever came out
 #pragma unroll
@@ -861,11 +885,39 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     const uint32_t stage = r1_s + (half * 4 + quad) * 2048;           // the products have read the resident rows
     const long long at = KEY_ROWS ? t.k0 + r : t.q0 + tok;
     uint16_t* row = reinterpret_cast<uint16_t*>(p.out) + at * p.o_sr + head * p.o_sh;
-    ragged_store(lane_at + F::ACC, half * DP / 2, (half + 1) * DP / 2, filled, false, MODE == RB_DKV || MODE == RB_DV ? 1.f : p.scale, row, p.D, live, fp16, stage);
-    if (MODE == RB_DKV) {
-      uint16_t* row2 = reinterpret_cast<uint16_t*>(p.out2) + at * p.o2_sr + head * p.o2_sh;
-      ragged_store(lane_at + F::ACC2, half * DP / 2, (half + 1) * DP / 2, filled, false, p.scale, row2, p.D, live, fp16, stage);
+    const bool write = live && (turn == 0 || odd);
+    if (MODE == RB_DKV || MODE == RB_DV) {
+      if (turn == 0) ragged_store(lane_at + F::ACC, half * DP / 2, (half + 1) * DP / 2, filled, false, 1.f, row, p.D, live, fp16, stage);
     }
+    if (F::DPROD) {
+      if (MODE == RB_DKV) row = reinterpret_cast<uint16_t*>(p.out2) + at * p.o2_sr + head * p.o2_sh;
+      odd = ragged_store<AGAIN>(lane_at + (MODE == RB_DKV ? F::ACC2 : F::ACC), half * DP / 2, (half + 1) * DP / 2, filled, false,
+                                AGAIN ? p.scale / lift : p.scale, row, p.D, write, fp16, stage) && live;
+    }
+  }
+  if (!AGAIN) break;
+  fence_proxy_async_smem();                 // copies may overwrite the stages
+  tc_fence_before();
+  const bool some = __syncthreads_or(odd);
+  tc_fence_after();
+  if (!some || turn == 1 || *abort_flag) break;
+  // the barriers start anew, once the last arrivals at those of emptied stages are there
+  if (warp == 1) {
+    auto last_phase = [&](int first, int stages) {
+      for (int st = 0; st < stages && st < blocks; ++st)
+        mbar_wait_warp(bar(first + st), ((blocks - 1 - st) / stages) & 1, abort_flag, p.err, ERR_WAIT_EMPTY);
+    };
+    last_phase(F::B_1E, F::S1);
+    if (!F::JOINT) last_phase(F::B_2E, F::S2);
+  }
+  __syncthreads();
+  if (*abort_flag) break;
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < F::BARS; ++i) mbar_inval(bar(i));
+    init_barriers();
+  }
+  __syncthreads();
+  lift = 1.f / 67108864.f;
   }
 
   if (*abort_flag) {                        // copies in flight land before the shared memory is given back

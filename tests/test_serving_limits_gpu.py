@@ -175,6 +175,30 @@ def test_ragged_a_query_that_is_no_number(dim, dtype, window):
     assert torch.equal(got[others], clean[others])
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("size", [1.0, 1e3, 1e5, 1e6])
+def test_ragged_fp16_gradients_of_large_scores(dim, size):
+    """fp16: gradients of scores beyond 65504 whose products with small keys and queries are within the type, beside rows of ordinary
+    size. The bound's last term: weights of 2^26 times the type's smallest half step, 2^-25, in rows that need the wider range."""
+    lens = [70, 5, 300, 131]
+    at = plain.starts(lens)
+    q, k, v, do = (rnd(at[-1], h, dim, seed=i, dtype=FP16) for i, h in enumerate((4, 2, 2, 4)))
+    large = slice(at[2], at[3])
+    k[large] *= 2.0 ** -10
+    q[large] *= 2.0 ** -10
+    v[large] *= size ** 0.5
+    do[at[2] + 1:at[3]] *= size ** 0.5
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.ragged_attention(*leaves, ints(*at)), leaves, do)
+    (_, (dq, eq), (dk, ek), (dv, ev)) = plain.ragged(q, k, v, at, at, None, dim ** -0.5, do)
+    room = torch.zeros(at[-1], dtype=torch.float64, device="cuda")
+    room[large] = 2.0 * lens[2] * 2 * dim ** -0.5 if size > 1 else 0.0          # two heads' sums of up to 300 weights off by up to 2
+    most = lambda t: room[:, None, None] * t[large].double().abs().amax()  # noqa: E731
+    for got, w, b in zip(grads, (dq, dk, dv), (eq + most(k), ek + most(q), ev)):
+        assert w.abs().max() < 60000
+        plain.near(got, w, b)
+
+
 def test_ragged_under_function_transforms():
     """Forward-mode derivatives and ``torch.func.grad`` against those of the double-precision formula; never a silent zero. Sums are 32-bit, the
     result is rounded to fp16: half a step is 2^-11 of a value."""
