@@ -244,10 +244,12 @@ class GenerationMixin:
                 return self._graph_greedy(input_ids, max_length, pad_token_id, eos_token_id, return_dict_in_generate)
             return self.greedy_search(input_ids, procs, stops, **common, **model_kwargs)
         if num_beams == 1 and do_sample:
-            warper = self._get_logits_warper(top_k, top_p, temperature, num_beams, min_p)
+            # a subclass may override both; it is handed what it may not know only where a caller asked for it
+            warper = self._get_logits_warper(top_k, top_p, temperature, num_beams, *((min_p,) if min_p else ()))
             input_ids, model_kwargs = self._expand_inputs_for_generation(input_ids, num_return_sequences, **model_kwargs)
-            fused = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p or 0.0) if fused_sampling else None
-            return self.sample(input_ids, procs, stops, warper, fused_settings=fused, **common, **model_kwargs)
+            if fused_sampling:
+                common["fused_settings"] = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p or 0.0)
+            return self.sample(input_ids, procs, stops, warper, **common, **model_kwargs)
         if min_p:
             raise ValueError("min_p belongs to sampling with one beam")
         bsz = input_ids.shape[0]

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import oslo_b200 as ob
 from oslo_b200 import ops
 
 
@@ -59,3 +60,28 @@ def test_ragged_statement_without_rows_or_keys():
         o = ops.ragged_attention(*leaves, ints(*starts), ints(*key_starts))
         assert o.shape == leaves[0].shape and o.isfinite().all() and not o[1:].any()
         assert all(g.isfinite().all() for g in torch.autograd.grad(o.sum(), leaves))
+
+
+def tiny(cls=None):
+    torch.manual_seed(0)
+    return (cls or ob.GPT2LMHeadModel)(ob.GPT2Config(vocab_size=61, n_positions=64, n_embd=32, n_layer=2, n_head=2)).eval()
+
+
+def test_generate_calls_overridden_steps_as_it_did():
+    """Subclasses that were written before ``min_p`` and ``fused_sampling`` are not handed what they do not know."""
+    class Older(ob.GPT2LMHeadModel):
+        @staticmethod
+        def _get_logits_warper(top_k, top_p, temperature, num_beams):
+            return ob.GPT2LMHeadModel._get_logits_warper(top_k, top_p, temperature, num_beams)
+
+        def sample(self, input_ids, logits_processor=None, stopping_criteria=None, logits_warper=None, pad_token_id=None, eos_token_id=None,
+                   output_scores=False, return_dict_in_generate=False, synced_gpus=False, **model_kwargs):
+            return super().sample(input_ids, logits_processor, stopping_criteria, logits_warper, pad_token_id, eos_token_id, output_scores,
+                                  return_dict_in_generate, synced_gpus, **model_kwargs)
+
+    ids = torch.arange(6).view(2, 3)
+    outs = []
+    for model in (tiny(), tiny(Older)):
+        torch.manual_seed(3)
+        outs.append(model.generate(ids, do_sample=True, max_length=12, top_k=9))
+    assert outs[0].tolist() == outs[1].tolist()
