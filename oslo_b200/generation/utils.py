@@ -248,7 +248,8 @@ class GenerationMixin:
             warper = self._get_logits_warper(top_k, top_p, temperature, num_beams, *((min_p,) if min_p else ()))
             input_ids, model_kwargs = self._expand_inputs_for_generation(input_ids, num_return_sequences, **model_kwargs)
             if fused_sampling:
-                common["fused_settings"] = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p or 0.0)
+                common["fused_settings"] = dict(temperature=1.0 if temperature is None else temperature, top_k=top_k or 0,
+                                                top_p=1.0 if top_p is None else top_p, min_p=min_p or 0.0)
             return self.sample(input_ids, procs, stops, warper, **common, **model_kwargs)
         if min_p:
             raise ValueError("min_p belongs to sampling with one beam")

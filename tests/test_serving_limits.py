@@ -85,3 +85,12 @@ def test_generate_calls_overridden_steps_as_it_did():
         torch.manual_seed(3)
         outs.append(model.generate(ids, do_sample=True, max_length=12, top_k=9))
     assert outs[0].tolist() == outs[1].tolist()
+
+
+@pytest.mark.parametrize("missing", ["temperature", "top_k", "top_p"])
+def test_fused_sampling_with_a_setting_that_the_config_leaves_out(missing):
+    model = tiny()
+    setattr(model.config, missing, None)
+    ids = torch.arange(6).view(2, 3)
+    assert model.generate(ids, do_sample=True, max_length=9).shape == (2, 9)
+    assert model.generate(ids, do_sample=True, max_length=9, fused_sampling=True).shape == (2, 9)
