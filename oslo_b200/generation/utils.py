@@ -355,7 +355,7 @@ class GenerationMixin:
             out, logits = self._step_logits(input_ids, model_kwargs)
             s = procs(input_ids, logits)
             if fused_settings is not None:
-                nxt = ops.sample_tokens(s, torch.rand(s.size(0), device=s.device), **fused_settings)
+                nxt = ops.sample_tokens(s, torch.rand(s.size(0), dtype=torch.float32, device=s.device), **fused_settings)
                 if bool((nxt < 0).any()):
                     raise RuntimeError("the logits hold no token to sample: not a number, or all minus infinity")
             if fused_settings is None or scores is not None:

@@ -94,3 +94,12 @@ def test_fused_sampling_with_a_setting_that_the_config_leaves_out(missing):
     ids = torch.arange(6).view(2, 3)
     assert model.generate(ids, do_sample=True, max_length=9).shape == (2, 9)
     assert model.generate(ids, do_sample=True, max_length=9, fused_sampling=True).shape == (2, 9)
+
+
+def test_fused_sampling_whatever_the_default_type():
+    model = tiny()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        assert model.generate(torch.arange(6).view(2, 3), do_sample=True, max_length=9, fused_sampling=True).shape == (2, 9)
+    finally:
+        torch.set_default_dtype(torch.float32)
