@@ -16,12 +16,16 @@ class PagedKVCache:
     ``extend([n_0, n_1, ...])`` makes room for that many more tokens per row and counts them; every layer then ``append``s their keys and
     values, and reads: ``attend`` for single tokens, ``read`` and ``ops.ragged_attention`` for prompts. ``release(row)`` gives a row's
     pages back. ``lengths`` and ``table`` are the device's copies, updated in place, so a captured step that reads them keeps doing so;
-    pages are handed out on the host, before the step. ``max_length``: tokens a row can hold (default: all pages)."""
+    pages are handed out on the host, before the step. ``max_length``: tokens a row can hold (default: all pages). ``dtype``: the keys' and
+    values' type, 16-bit on a GPU."""
 
     def __init__(self, layers: int, pages: int, page: int, heads: int, dim: int, rows: int, dtype: torch.dtype = torch.bfloat16,
                  device=None, quantised: bool = False, max_length: Optional[int] = None) -> None:
         if min(layers, pages, page, heads, dim, rows) <= 0:
             raise ValueError("PagedKVCache: sizes must be positive")
+        where = torch.get_default_device() if device is None else torch.device(device)
+        if where.type == "cuda" and (dtype not in (torch.bfloat16, torch.float16) or dim > 256 or dim % (16 if quantised else 8)):
+            raise ValueError("PagedKVCache: on a GPU keys and values are bf16 or fp16, in heads of a multiple of 8 (quantised: 16) values up to 256")
         store = torch.float8_e4m3fn if quantised else dtype
         shape = (pages, heads, page, dim)
         # zeros in bytes: not every operator exists for 8-bit floats

@@ -4,6 +4,7 @@ import torch
 
 import oslo_b200 as ob
 from oslo_b200 import ops
+from oslo_b200.generation import PagedKVCache
 
 
 def rnd(*shape, seed=0, dtype=torch.float32):
@@ -103,3 +104,10 @@ def test_fused_sampling_whatever_the_default_type():
         assert model.generate(torch.arange(6).view(2, 3), do_sample=True, max_length=9, fused_sampling=True).shape == (2, 9)
     finally:
         torch.set_default_dtype(torch.float32)
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=torch.float32), dict(dtype=torch.float32, quantised=True), dict(dim=20), dict(dim=264), dict(dim=24, quantised=True)])
+def test_a_cache_that_the_kernels_cannot_fill_is_refused_when_it_is_made(bad):
+    with pytest.raises(ValueError, match="GPU"):
+        PagedKVCache(**dict(dict(layers=1, pages=4, page=8, heads=2, dim=64, rows=2, device="cuda"), **bad))
+    PagedKVCache(**dict(dict(layers=1, pages=4, page=8, heads=2, dim=64, rows=2, device="cpu"), **bad))
