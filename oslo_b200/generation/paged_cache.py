@@ -21,7 +21,7 @@ class PagedKVCache:
 
     def __init__(self, layers: int, pages: int, page: int, heads: int, dim: int, rows: int, dtype: torch.dtype = torch.bfloat16,
                  device=None, quantised: bool = False, max_length: Optional[int] = None) -> None:
-        if min(layers, pages, page, heads, dim, rows) <= 0:
+        if min(layers, pages, page, heads, dim, rows) <= 0 or (max_length is not None and max_length <= 0):
             raise ValueError("PagedKVCache: sizes must be positive")
         where = torch.get_default_device() if device is None else torch.device(device)
         if where.type == "cuda" and (dtype not in (torch.bfloat16, torch.float16) or dim > 256 or dim % (16 if quantised else 8)):
@@ -34,7 +34,8 @@ class PagedKVCache:
         self.k, self.v = [make() for _ in range(layers)], [make() for _ in range(layers)]
         self.k_scale, self.v_scale = [scale() for _ in range(layers)], [scale() for _ in range(layers)]
         self.page, self.dtype = page, dtype
-        columns = pages if max_length is None else min(pages, -(-max_length // page))
+        self.max_length = pages * page if max_length is None else min(pages * page, max_length)
+        columns = self._pages(self.max_length)
         self.table = torch.full((rows, columns), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=device)
         self._table = torch.full((rows, columns), -1, dtype=torch.int32)
@@ -53,12 +54,15 @@ class PagedKVCache:
         self.lengths.copy_(torch.tensor(self._lengths, dtype=torch.int32))
 
     def extend(self, new: Sequence[int]) -> None:
-        """Room for ``new[r]`` more tokens of row ``r``. Refuses, and changes nothing, where pages run out."""
+        """Room for ``new[r]`` more tokens of row ``r``. Refuses, and changes nothing, where pages run out or a row would be longer than
+        ``max_length``."""
         if len(new) != len(self._lengths) or any(n < 0 for n in new):
             raise ValueError(f"PagedKVCache: {len(self._lengths)} rows, {len(new)} numbers of new tokens")
         then = [a + int(n) for a, n in zip(self._lengths, new)]
         need = [self._pages(t) - self._pages(a) for t, a in zip(then, self._lengths)]
-        if sum(need) > len(self._free) or any(self._pages(t) > self._table.size(1) for t in then):
+        if max(then) > self.max_length:
+            raise RuntimeError(f"KV cache overflow: {max(then)} tokens in a row, which holds {self.max_length}")
+        if sum(need) > len(self._free):
             raise RuntimeError(f"KV cache overflow: {sum(need)} more pages, {len(self._free)} are free")
         for r, n in enumerate(need):
             at = self._pages(self._lengths[r])

@@ -111,3 +111,15 @@ def test_a_cache_that_the_kernels_cannot_fill_is_refused_when_it_is_made(bad):
     with pytest.raises(ValueError, match="GPU"):
         PagedKVCache(**dict(dict(layers=1, pages=4, page=8, heads=2, dim=64, rows=2, device="cuda"), **bad))
     PagedKVCache(**dict(dict(layers=1, pages=4, page=8, heads=2, dim=64, rows=2, device="cpu"), **bad))
+
+
+def test_a_row_holds_max_length_tokens_and_no_more():
+    cache = PagedKVCache(layers=1, pages=9, page=4, heads=1, dim=16, rows=2, dtype=torch.float32, max_length=10)
+    cache.extend([9, 3])
+    with pytest.raises(RuntimeError, match="10"):
+        cache.extend([2, 0])
+    assert cache.lengths.tolist() == [9, 3] and cache.free_pages == 5
+    cache.extend([1, 7])
+    assert cache.lengths.tolist() == [10, 10]
+    with pytest.raises(ValueError):
+        PagedKVCache(layers=1, pages=9, page=4, heads=1, dim=16, rows=2, max_length=0)
