@@ -38,7 +38,7 @@ class PagedKVCache:
         columns = self._pages(self.max_length)
         self.table = torch.full((rows, columns), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=device)
-        self._table = torch.full((rows, columns), -1, dtype=torch.int32)
+        self._table = torch.full((rows, columns), -1, dtype=torch.int32, device="cpu")
         self._lengths: List[int] = [0] * rows
         self._free = list(range(pages - 1, -1, -1))
 
@@ -51,7 +51,7 @@ class PagedKVCache:
 
     def _publish(self) -> None:
         self.table.copy_(self._table)
-        self.lengths.copy_(torch.tensor(self._lengths, dtype=torch.int32))
+        self.lengths.copy_(torch.tensor(self._lengths, dtype=torch.int32, device="cpu"))
 
     def extend(self, new: Sequence[int]) -> None:
         """Room for ``new[r]`` more tokens of row ``r``. Refuses, and changes nothing, where pages run out or a row would be longer than

@@ -123,3 +123,14 @@ def test_a_row_holds_max_length_tokens_and_no_more():
     assert cache.lengths.tolist() == [10, 10]
     with pytest.raises(ValueError):
         PagedKVCache(layers=1, pages=9, page=4, heads=1, dim=16, rows=2, max_length=0)
+
+
+def test_pages_are_handed_out_on_the_host_whatever_the_default_device():
+    torch.set_default_device("meta")
+    try:
+        cache = PagedKVCache(layers=1, pages=6, page=4, heads=1, dim=16, rows=2, dtype=torch.float32, device="cpu")
+        cache.extend([5, 1])
+        cache.release(0)
+    finally:
+        torch.set_default_device(None)
+    assert cache.lengths.tolist() == [0, 1] and cache.free_pages == 5
