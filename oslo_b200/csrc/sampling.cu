@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleParam
     sp_sync<C>();                                               // nobody leaves while another reads its shared memory
     return;
   }
-  if (!(temperature > 0.0) || top_k == 1 || top_p <= 0.0) {     // the first of the largest
+  if (!(temperature > 0.0) || top_k == 1 || !(top_p > 0.0) || min_p != min_p) {      // the first of the largest
     u64 best = ~0ull;
     each([&](float v, int at) {
       if (v == m) best = sp_min(best, first + at);

@@ -446,9 +446,10 @@ def sample_tokens(logits: Tensor, uniform: Tensor, temperature=1.0, top_k=0, top
     Tokens are ranked by logit, equal ones by index. With ``w = exp((logit - largest) / temperature)``: ``top_k`` (0: all) keeps that
     many ranks, ``top_p`` those of them whose lower ranks have at most this share of their mass, ``min_p`` tokens of at least this
     ``w``; rank 0 always stays. The first token, by index, whose kept mass together with its predecessors' exceeds ``uniform`` times
-    the whole is the choice. Every setting is a number or a tensor ``[rows]`` (fp32; ``top_k`` int32). A temperature of 0 takes the
-    largest logit; on a GPU a token of less than 2^-46 of the largest ``w`` is never chosen. A row whose logits hold no number to choose
-    (one that is no number, or only minus infinities), or whose ``uniform`` is outside ``[0, 1)``, gives -1. No gradients."""
+    the whole is the choice. Every setting is a number or a tensor ``[rows]`` (fp32; ``top_k`` int32). A temperature of 0, and a row's
+    setting that is no number, takes the largest logit; on a GPU a token of less than 2^-46 of the largest ``w`` is never chosen. A row whose
+    logits hold no number to choose (one that is no number, or only minus infinities), or whose ``uniform`` is outside ``[0, 1)``,
+    gives -1. No gradients."""
     for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
         if not isinstance(value, Tensor) and not value >= 0:
             raise ValueError(f"sample_tokens: {name} must not be negative")

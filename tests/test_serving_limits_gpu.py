@@ -119,6 +119,17 @@ def test_sampling_logits_far_larger_than_the_temperature(given, dtype, temperatu
     assert torch.equal(ops.sample_tokens(x, u, temperature=temperature, **given), want)
 
 
+def test_sampling_settings_that_are_no_numbers():
+    """Per row: the first of the largest logits, on a GPU as on the CPU."""
+    x, u = rnd(12, 3001, seed=3), torch.full((12,), 0.9, device="cuda")
+    x[:, 5] = x[:, 77] = 9.0
+    nan = torch.full((12,), float("nan"), device="cuda")
+    for given in (dict(temperature=nan), dict(top_p=nan), dict(min_p=nan), dict(top_p=nan, top_k=900), dict(min_p=nan, top_k=40)):
+        full = settings_of(**given)
+        assert (ops.sample_tokens(x, u, **given) == 5).all()
+        assert (ops.reference.sample_tokens(x.cpu(), u.cpu(), **{k: v.cpu() if torch.is_tensor(v) else v for k, v in full.items()}) == 5).all()
+
+
 # ------------------------------------------------------------------------------------------------------------------ packed attention
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
