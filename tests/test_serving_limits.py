@@ -5,6 +5,7 @@ import torch
 import oslo_b200 as ob
 from oslo_b200 import ops
 from oslo_b200.generation import PagedKVCache
+from oslo_b200.ops.cuda_ops import _op
 
 
 def rnd(*shape, seed=0, dtype=torch.float32):
@@ -29,7 +30,7 @@ def test_ragged_gradients_of_a_trace_have_their_strides(joint):
             k = k.contiguous()
         at = torch.empty(4, dtype=torch.int32, device="cuda")
         do, o, lse = torch.empty_like(q), torch.empty_like(q), torch.empty(rows, heads, device="cuda")
-        got = torch.ops.oslo_b200.ragged_bwd(do, q, k, v, o, lse, at, at, 0.125, 0)
+        got = _op("ragged_bwd")(do, q, k, v, o, lse, at, at, 0.125, 0)
         for g, t in zip(got, (q, k, v)):
             assert g.shape == t.shape and g.dtype == t.dtype
             assert g.stride() == (t.stride() if joint else (t.size(1) * dim, dim, 1))
