@@ -223,8 +223,9 @@ static int paged_move(const PagedMove& p, int dtype, bool q8, int sms, cudaStrea
 // The products of 16 keys with 8 query heads (NB = 2: 16) run on mma.sync - m16n8k16 with the keys as its 16 rows is as small as one
 // token's work gets; tcgen05's 128 rows would be 8 to 128 times more than there is - and stay far below the memory's pace.
 //   S^T = K q^T: K straight from the queue (ldmatrix). A weight's reference follows the running maximum only when a score has outgrown
-//   it by 2^8, so a step usually needs one vote and no exchange. P^T is rounded to the pool's type and turned by movmatrix into the
-//   right operand of O^T = V^T P^T.
+//   it by 2^8, so a step usually needs one vote and no exchange. P^T is rounded to the pool's type, since the products take two operands of
+//   one 16-bit type (half a step: 2^-8 of a weight in bf16, 2^-11 in fp16, as for the result itself; e4m3 pools: f16, 2^-11), and turned by
+//   movmatrix into the right operand of O^T = V^T P^T.
 //   8-bit pools: four e4m3 bytes of ldmatrix's 32 bits become two f16 pairs. The column index inside the first product and the rows of
 //   the second are permuted so that no byte moves between lanes; q (divided by a power of two per head: f16 then holds it) is permuted
 //   alike, and the value scales go into P, relative to the largest seen so far or a sixteenth of it.

@@ -13,10 +13,11 @@
 //   dK, dV   rows = keys      S^T = K Q^T, dP^T = V dO^T   P^T, dS^T = P^T o (dP - delta)   dV += P^T dO, dK += dS^T Q
 //   dQ       rows = queries   S = Q K^T, dP = dO V^T       dS = P o (dP - delta)        dQ += dS K
 //
-// P is rounded to the inputs' type for its products (half a step: 2^-9 of a weight, or 2^-12 in fp16), as the results are. dS, a difference,
-// goes into its products as two numbers of that type: rounded to one, dQ and dK were 1.5 (bf16) to 1.9 (fp16) times as far from the formula
-// as their own rounding puts them, now 1.1 to 1.4 times; it costs 5 % of the backward pass with heads of 128. Maxima, sums and all
-// accumulators are 32-bit.
+// P is rounded to the inputs' type for its products, since the tensor core multiplies numbers of one 16-bit type: half a step is 2^-8 of a
+// weight in bf16 and 2^-11 in fp16, as for the results themselves, and two numbers a weight would double the products of P V. With that
+// outputs are 1.25 to 1.4 times as far from the formula as one rounding at the end puts them. dS, a difference, goes into its products as
+// two numbers of that type: rounded to one, dQ and dK were 1.5 (bf16) to 1.9 (fp16) times as far off, now 1.1 to 1.4 times; it costs 5 % of
+// the backward pass with heads of 128. Maxima, sums and all accumulators are 32-bit.
 //
 // Not in the reference, which pads batches (oslo/models/gptj/modeling_gptj.py:151-191 is the attention of one).
 #include "attention_sm100.cuh"
@@ -234,7 +235,7 @@ __device__ __forceinline__ bool ragged_store(uint32_t acc, int from, int to, boo
 // MT tiles of 128 rows per CTA. D <= 128: two, with a softmax warpgroup each (thread = row), so that the tensor core works for one tile
 // while the other's exponentials run. S of two blocks of 64 keys per tile: Q K^T of the next block runs under the softmax of this one (with
 // blocks of 128 keys TMEM holds one S a tile; its Q K^T then waited for P V: 350 us instead of 298 for 2 x 4096 tokens, 32/8 heads of
-// 128). P overwrites S. Warp 0: TMA; a warp a tile issues its products; then a warpgroup a tile for the softmax. A wait that is over at once
+// 128, which take 261 since the results pass through shared memory). P overwrites S. Warp 0: TMA; a warp a tile issues its products; then a warpgroup a tile for the softmax. A wait that is over at once
 // still takes 100 to 200 cycles and a commit not much less, so an issuer has two of each a block: K of the next block and V of this one
 // share a stage (with one warp for both tiles and five waits and commits a tile: 449 us).
 template <int DP> struct RaggedFwd {
@@ -242,8 +243,8 @@ template <int DP> struct RaggedFwd {
   static constexpr int FIRST = 1 + MT, THREADS = 32 * (FIRST + 4 * MT), ROWS = 128 * MT;      // FIRST: the first softmax warp
   static constexpr int DC = DP / 64;
   // of 8 pairs of exponentials, those that the FMA pipe computes: 16 a clock come from the special function unit, half of a block's time.
-  // 0, 1, 2, 3 of 8, measured before the results went through shared memory: 315, 305, 304, 305 us for heads of 128, 285, 277, 275, 276
-  // for 64, 521, 525, 535, 539 for 256 (one tile: its products wait for its softmax, and the polynomial's longer chain shows)
+  // 0, 1, 2, 3 of 8, 2 x 4096 tokens, 32/8 heads: 268, 285, 261, 271 us for heads of 128, 264, 263, 254, 253 for 64; 0 and 2 of 8: 498, 510
+  // for 256 (one tile: its products wait for its softmax, and the polynomial's longer chain shows)
   static constexpr int FMA_EXP = DP <= 128 ? 2 : 0;
   static constexpr uint32_t Q_SUB = 128 * 128, Q_TILE = DC * Q_SUB, KV_SUB = BN * 128, KV_TILE = DC * KV_SUB;
   static constexpr int STAGES = DP == 256 ? 2 : (DP == 128 ? 4 : 6);       // of K of block j + 1 and V of block j
@@ -521,7 +522,8 @@ ragged_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
 
 // ---------------------------------------------------------------------------------------------------------------- backward
 // What the other kernels need of a query row: its log-sum-exp in log2 units and delta[t, h] = sum_d dO O in 32 bits, negative, side by side; DP / 8
-// lanes a row. Bound by reading both.
+// lanes a row. Bound by reading both. O is the rounded output: that moves delta by up to half a step of each term (2^-8 in bf16, 2^-11 in fp16),
+// as it moves everything else that is made of the output; an output in 32 bits kept for this would double what the forward pass writes.
 template <typename T, int LPR>
 __global__ void __launch_bounds__(256) ragged_delta_kernel(const T* __restrict__ o, const T* __restrict__ g, const float* __restrict__ lse,
                                                            float2* __restrict__ stats, long long rows, int H, int D, long long o_sr, long long o_sh, long long g_sr,
@@ -557,7 +559,7 @@ enum : int { RB_DKV = 0, RB_DV = 1, RB_DK = 2, RB_DQ = 3 };
 // of the columns each: P and dS go back, packed, into the half they came from. Head sizes of 256 take dV and dK in two launches: both
 // accumulators fill TMEM alone. r1, s1: what S is made of; r2, s2: what dP (and dV) is made of.
 //
-// 2 x 4096 tokens, 32/8 heads: 1332 us with heads of 128, 1047 with 64, 3318 with 256 (a block of dK and dV takes 2240 cycles with 128, of
+// 2 x 4096 tokens, 32/8 heads: 1338 us with heads of 128, 993 with 64, 3290 with 256 (a block of dK and dV takes 2240 cycles with 128, of
 // which its products need 1540: S and dP have 64 columns, which the tensor core takes at three quarters of its rate, since both
 // operands come from shared memory). Per block one wait and one commit fewer (JOINT), the statistics brought by a warp of their own and a
 // uniform test for blocks without a mask: 1278 instead of 1450, before dS became two numbers. Exponentials on the FMA pipe do not pay here (1408 instead of 1363): the

@@ -623,8 +623,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleParam
     for (int i = tid; i < SP_BINS; i += SP_THREADS) s.count[i] = 0;
     __syncthreads();
     // top-p's whole in the same pass: its 64-bit exponentials run while the histogram's atomics wait (512 rows of 50400, top-p 0.9: 107 us.
-    // 32-bit ones take 88, but are off by 2^-21, which moves the last token kept in one row of ten; a bound on that error, and the rest of the row
-    // weighed only where the border is nearer, 102 to 106, and 250 instead of 220 at a temperature of 2)
+    // 32-bit ones take 88, but are off by 2^-21, which moves the last token kept in some rows of a hundred; a bound on that error, and the rest
+    // of the row weighed only where the border is nearer, 102 to 106, and 250 instead of 220 at a temperature of 2)
     const bool weighed = by_p && !by_k;
     for (int j = j0 + lane; j < j1; j += 32) {
       float v[PER];
